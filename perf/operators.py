@@ -239,8 +239,8 @@ def prepare(case, seed):
         _scatter(st["token"], tok, table, page)
         # the pages' other planes are not read
         for name, x in (("k", D), ("v", D), ("b", S)):
-            st[name] = torch.zeros((1, 1, 1, x), dtype=torch.bfloat16, device=dev).expand(P, H, page, x)
-        st["g"] = st["f"] = st["weight"]
+            st[name] = torch.empty((P, H, page, x), dtype=torch.bfloat16, device=dev)
+        st["g"], st["f"] = torch.empty_like(st["weight"]), torch.empty_like(st["weight"])
     elif op == "append":
         dt, page, budget = DTYPES[case["dtype"]], case["page"], case["budget"]
         n = budget if budget else 96
