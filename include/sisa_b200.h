@@ -355,6 +355,86 @@ int sisa_decode_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q,
                      int64_t B, int64_t H, int64_t N, int dtype, const sisa_view4* y, void* workspace,
                      int32_t* status, void* stream);
 
+/* ---- paged cache (a server's form of the decode cache of src/sisa/generation.py:58-95, which holds one
+ * rectangular batch): the keys of every sequence lie in pages of page_size slots, and the number of keys
+ * kept per sequence can be bounded, the keys with the least accumulated attention weight going first. A
+ * key's position is carried by its g, F and rotated b~, so the slots may hold the keys in any order.
+ *
+ * sisa_pages: one layer's pages. k, v (n_pages, H, page_size, 64) and b (n_pages, H, page_size, 32) in the
+ * call's 16-bit dtype, g, f, weight (accumulated attention weight) and token (index of the token in its
+ * sequence) (n_pages, H, page_size) in 32 bits; page and head strides in elements (k_sp, k_sh, ...; s_sp and
+ * s_sh for the four planes), the rows of one head in one page dense, 16-byte aligned. page_size 16, 32, 64,
+ * 128 or 256. f may be NULL without a forget gate; weight and token where nothing is evicted.
+ * table: (B, max_pages) int32, row stride table_sb: the page of each block of page_size slots of a
+ * sequence. Entries are read only where a slot is used; one outside [0, n_pages) sets SISA_ST_BAD_POS and
+ * its keys are left out. B*H <= 65,535. */
+typedef struct sisa_pages {
+  void* k;
+  void* v;
+  void* b;
+  float* g;
+  float* f;
+  float* weight;
+  int32_t* token;
+  int64_t k_sp, k_sh, v_sp, v_sh, b_sp, b_sh, s_sp, s_sh;
+  int64_t n_pages, page_size;
+} sisa_pages;
+
+/* One new query row per (sequence, head) against that sequence's lengths[b] keys (slots 0 .. lengths[b] - 1):
+ *   s_j = q.k_j/8 + lam_h exp(min(g_q - g_j, 0)) (c.b_j) + (F_q - F_j), y = softmax(s) v, in fp32.
+ * q (B, H, 1, 64), c (B, H, 1, 32) views in `dtype`; g_q, f_q (B, H) fp32 contiguous (f_q NULL: no forget gate);
+ * lengths (B,) int32; y (B, H, 1, 64) view; lse (B, H) fp32 in log2 units, or NULL. With weight_out (a plane
+ * with the strides of pages->weight, which it may be) every key's share is added:
+ * weight_out_j = weight_j + softmax(s)_j; slots past a sequence's length are not written. A sequence of
+ * length <= 0 gives y = 0 and lse = -inf; a length above max_pages * page_size is cut there and sets
+ * SISA_ST_BAD_POS. workspace: sisa_paged_attn_workspace(B, H, max_pages * page_size, weight_out != NULL)
+ * bytes, 16-byte aligned, one call at a time. Deterministic. */
+int64_t sisa_paged_attn_workspace(int64_t B, int64_t H, int64_t max_keys, int accumulate);
+int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, const float* f_q,
+                    const sisa_pages* pages, const int32_t* table, int64_t table_sb, int64_t max_pages,
+                    const int32_t* lengths, const float* lam, int64_t B, int64_t H, int dtype, const sisa_view4* y,
+                    float* lse, float* weight_out, void* workspace, int32_t* status, void* stream);
+
+/* The slot whose key the token `position[b]` (int32, its index in the sequence; < 0: idle row) replaces:
+ * slots[b, h] = the slot j < budget of the least weight among the keys with token_j < position[b] - recent
+ * (the `recent` newest stay), the lowest slot where several weigh the same, a NaN weight before all others;
+ * -1 while position[b] < budget (nothing has to go yet). 0 <= recent < budget <= max_pages * page_size. */
+int sisa_paged_evict(const sisa_pages* pages, const int32_t* table, int64_t table_sb, int64_t max_pages,
+                     const int32_t* position, int64_t B, int64_t H, int64_t budget, int64_t recent, int32_t* slots,
+                     int32_t* status, void* stream);
+
+/* sisa_decode_prep on pages: the token `position[b]` of every sequence from its fused projection row, with the
+ * recurrences in a state of their own: carry (B, H, 18) fp32 {Phi 0..15, g, F} of the previous token (zero before
+ * the first), read from carry_in and written to carry_out (which may be the same). The key goes to slot
+ * slots[b, h] where slots is given and that is >= 0, else to slot position[b]; its weight becomes 0 and its
+ * token position[b]. lengths (optional): min(position[b] + 1, budget), budget 0 meaning no bound. A slot at or
+ * past the budget (without one, max_pages * page_size) sets SISA_ST_BAD_POS. Such a row, and an idle one
+ * (position[b] < 0; its length is 0), writes no key, keeps its carry and has c_out, g_out and f_out 0. */
+int sisa_paged_append(const void* proj, int64_t proj_sb, const float* z, int64_t z_sb, const sisa_pages* pages,
+                      const int32_t* table, int64_t table_sb, int64_t max_pages, const int32_t* position,
+                      const int32_t* slots, int64_t budget, int64_t B, int64_t H, int dtype, const float* carry_in,
+                      float* carry_out, void* c_out, float* g_out, float* f_out, int32_t* lengths, int32_t* status,
+                      void* stream);
+
+/* The attention each prompt key received: w[b, h, j] = sum over queries i in [max(j, first_query), L) of
+ * softmax(s_i)_j = 2^(s_ij log2e - lse_i), with the operands of sisa_attn_fwd and the lse (log2 units) it wrote
+ * (rows from first_query on are read). w (B, H, L) fp32 contiguous. first_query in [0, L): 0 takes all queries. */
+int sisa_attn_key_weights(const sisa_view4* q, const sisa_view4* k, const sisa_view4* c, const sisa_view4* b,
+                          const float* pos, const float* lam, const float* lse, int64_t B, int64_t H, int64_t L,
+                          int64_t first_query, int dtype, float* w, int32_t* status, void* stream);
+
+/* A prompt's keys into pages: of the L positions of every (sequence, head), the `recent` newest and the
+ * keep - recent others of the largest weight (the earlier position where two weigh the same, a NaN weight
+ * last), in ascending order into slots 0 .. keep - 1, with their g, f, weight (0 without weight) and token.
+ * k, v (B, H, L, 64) and b (B, H, L, 32) views; g, f (B, H, L) fp32 with strides g_sb, g_sh and unit stride
+ * along L (f NULL: zeros); weight (B, H, L) fp32 contiguous, or NULL with keep == L. Planes that the pages
+ * lack are not written. 0 <= recent <= keep <= L. workspace: sisa_paged_fill_workspace(B, H, keep) bytes. */
+int64_t sisa_paged_fill_workspace(int64_t B, int64_t H, int64_t keep);
+int sisa_paged_fill(const sisa_pages* pages, const int32_t* table, int64_t table_sb, int64_t max_pages,
+                    const sisa_view4* k, const sisa_view4* v, const sisa_view4* b, const float* g, int64_t g_sb,
+                    int64_t g_sh, const float* f, int64_t f_sb, int64_t f_sh, const float* weight, int64_t B, int64_t H,
+                    int64_t L, int64_t keep, int64_t recent, void* workspace, int32_t* status, void* stream);
+
 /* Allocation-free variant of sisa_decode_attn (no counterpart in the reference): identical arguments
  * except that there is no workspace. For callers that cannot allocate device memory when they decode:
  * host programs that bind only this C ABI and have no device allocator, and serving loops held to a

@@ -78,6 +78,17 @@ class NormBwdArgs(ctypes.Structure):
                 ("dweight", _P), ("dproj_w", _P), ("dproj_b", _P),
                 ("workspace", _P)]
 
+
+class Pages(ctypes.Structure):
+    """``sisa_pages``: one layer's pages of a paged cache."""
+
+    _fields_ = [("k", _P), ("v", _P), ("b", _P), ("g", _P), ("f", _P), ("weight", _P), ("token", _P),
+                ("k_sp", _I64), ("k_sh", _I64), ("v_sp", _I64), ("v_sh", _I64), ("b_sp", _I64), ("b_sh", _I64),
+                ("s_sp", _I64), ("s_sh", _I64), ("n_pages", _I64), ("page_size", _I64)]
+
+
+_PGP = ctypes.POINTER(Pages)
+
 # name -> (restype, argtypes); every symbol declared in include/sisa_b200.h
 SIGNATURES = {
     "sisa_version": (ctypes.c_char_p, []),
@@ -124,6 +135,15 @@ SIGNATURES = {
                                    _P, _P, _P, _P]),
     "sisa_decode_attn_dpos": (_I, [_VP, _VP, _P, _P, _VP, _VP, _VP, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _I, _VP,
                                    _P, _P, _P]),
+    "sisa_paged_attn_workspace": (_I64, [_I64, _I64, _I64, _I]),
+    "sisa_paged_attn": (_I, [_VP, _VP, _P, _P, _PGP, _P, _I64, _I64, _P, _P, _I64, _I64, _I, _VP, _P, _P, _P, _P, _P]),
+    "sisa_paged_evict": (_I, [_PGP, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "sisa_paged_append": (_I, [_P, _I64, _P, _I64, _PGP, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _P,
+                               _P, _P, _P, _P]),
+    "sisa_attn_key_weights": (_I, [_VP, _VP, _VP, _VP, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "sisa_paged_fill_workspace": (_I64, [_I64, _I64, _I64]),
+    "sisa_paged_fill": (_I, [_PGP, _P, _I64, _I64, _VP, _VP, _VP, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64,
+                             _I64, _I64, _P, _P, _P]),
     "sisa_rmsnorm_bwd_workspace": (_I64, [_I64, _I64]),
     "sisa_rmsnorm_fwd": (_I, [_P, _I64, _I, _P, _I64, _I64, ctypes.c_float, _P, _I64, _I, _P, _P, _P]),
     "sisa_rmsnorm_bwd": (_I, [_P, _I64, _I, _P, _I64, _I, _P, _P, _I64, _I64, _P, _I64, _I, _P, _P, _P, _P]),

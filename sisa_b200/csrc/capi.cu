@@ -21,6 +21,7 @@
 #include "copy.h"
 #include "embed.h"
 #include "norm.h"
+#include "key_weights.h"
 #include "capi_util.h"
 
 namespace {
@@ -387,6 +388,31 @@ int sisa_attn_bwd(const sisa_view4* q, const sisa_view4* k, const sisa_view4* v,
   p.status = status;
   cudaError_t e = sisa::launch_attn_bwd(p, dtype, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? SISA_OK : cuda_fail(e, "sisa_attn_bwd launch");
+}
+
+int sisa_attn_key_weights(const sisa_view4* q, const sisa_view4* k, const sisa_view4* c, const sisa_view4* b,
+                          const float* pos, const float* lam, const float* lse, int64_t B, int64_t H, int64_t L,
+                          int64_t first_query, int dtype, float* w, int32_t* status, void* stream) {
+  int rc;
+  if ((rc = check_dims(B, H, L)) || (rc = check_dtype(dtype))) return rc;
+  if ((rc = check_view(q, 2, "q")) || (rc = check_view(k, 2, "k")) || (rc = check_view(c, 2, "c")) ||
+      (rc = check_view(b, 2, "b")))
+    return rc;
+  if (!pos || !lam || !lse || !w) return fail(SISA_ERR_VALUE, "sisa_attn_key_weights: null pos, lam, lse or w");
+  if (!aligned16(pos)) return fail(SISA_ERR_ALIGN, "sisa_attn_key_weights: pos must be 16-byte aligned");
+  if (first_query < 0 || first_query >= L)
+    return fail(SISA_ERR_VALUE, "sisa_attn_key_weights: first_query %lld outside [0, %lld)", (long long)first_query,
+                (long long)L);
+  sisa::KeyWeightParams p{};
+  p.q = static_cast<const char*>(q->data); p.q_sb = q->stride_b; p.q_sh = q->stride_h; p.q_sl = q->stride_l;
+  p.k = static_cast<const char*>(k->data); p.k_sb = k->stride_b; p.k_sh = k->stride_h; p.k_sl = k->stride_l;
+  p.c = static_cast<const char*>(c->data); p.c_sb = c->stride_b; p.c_sh = c->stride_h; p.c_sl = c->stride_l;
+  p.b = static_cast<const char*>(b->data); p.b_sb = b->stride_b; p.b_sh = b->stride_h; p.b_sl = b->stride_l;
+  p.pos = pos; p.lam = lam; p.lse = lse; p.w = w;
+  p.B = (int)B; p.H = (int)H; p.L = (int)L; p.Lp = (int)sisa_pos_len(L); p.first = (int)first_query;
+  p.status = status;
+  cudaError_t e = sisa::launch_key_weights(p, dtype, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SISA_OK : cuda_fail(e, "sisa_attn_key_weights launch");
 }
 
 int sisa_prep_bwd(const void* proj, int64_t B, int64_t L, int64_t H, int64_t proj_sb, int64_t proj_sl, int dtype,
