@@ -403,13 +403,20 @@ int sisa_attn_key_weights(const sisa_view4* q, const sisa_view4* k, const sisa_v
   if (first_query < 0 || first_query >= L)
     return fail(SISA_ERR_VALUE, "sisa_attn_key_weights: first_query %lld outside [0, %lld)", (long long)first_query,
                 (long long)L);
-  sisa::KeyWeightParams p{};
-  p.q = static_cast<const char*>(q->data); p.q_sb = q->stride_b; p.q_sh = q->stride_h; p.q_sl = q->stride_l;
-  p.k = static_cast<const char*>(k->data); p.k_sb = k->stride_b; p.k_sh = k->stride_h; p.k_sl = k->stride_l;
-  p.c = static_cast<const char*>(c->data); p.c_sb = c->stride_b; p.c_sh = c->stride_h; p.c_sl = c->stride_l;
-  p.b = static_cast<const char*>(b->data); p.b_sb = b->stride_b; p.b_sh = b->stride_h; p.b_sl = b->stride_l;
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(q->data))) return rc;
+  const CUtensorMapDataType dt = dtype == SISA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  sisa::KeyWeightParams p;
+  memset(&p, 0, sizeof(p));
+  if ((rc = map_view4(&p.tm_k, k, B, H, L, 64, 2, dt, 128, CU_TENSOR_MAP_SWIZZLE_128B, "k")) ||
+      (rc = map_view4(&p.tm_b, b, B, H, L, 32, 2, dt, 128, CU_TENSOR_MAP_SWIZZLE_64B, "b")) ||
+      (rc = map_view4(&p.tm_q, q, B, H, L, 64, 2, dt, 64, CU_TENSOR_MAP_SWIZZLE_128B, "q")) ||
+      (rc = map_view4(&p.tm_c, c, B, H, L, 32, 2, dt, 64, CU_TENSOR_MAP_SWIZZLE_64B, "c")) ||
+      (rc = map_records(&p.tm_pos, pos, B * H, L, sisa_pos_len(L), "pos")))
+    return rc;
   p.pos = pos; p.lam = lam; p.lse = lse; p.w = w;
   p.B = (int)B; p.H = (int)H; p.L = (int)L; p.Lp = (int)sisa_pos_len(L); p.first = (int)first_query;
+  p.ntk = (int)((L + 127) / 128);
   p.status = status;
   cudaError_t e = sisa::launch_key_weights(p, dtype, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? SISA_OK : cuda_fail(e, "sisa_attn_key_weights launch");

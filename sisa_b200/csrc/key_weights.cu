@@ -1,82 +1,227 @@
-// key_weights.cu - the attention each prompt key received:
+// key_weights.cu - the attention each prompt key received, on Blackwell tensor cores:
 //   w_j = sum over queries i in [max(j, first), L) of 2^(x_ij - lse_i),
 //   x_ij = log2e (q_i.k_j / 8 + lam_h exp(min(g_i - g_j, 0)) (c_i.b~_j) + (F_i - F_j)),
-// with lse from the attention forward. Every key is owned by one thread, which adds its queries in
-// order: no atomics.
+// with lse from the attention forward, so no running maximum is needed and every share is <= 1.
+//
+// CTA = 128 keys of one (batch, head), resident; it walks the 64-query tiles from its own diagonal (or from
+// first) to the end. Warp roles:
+//   warps 0-7  compute: a thread owns one key row (TMEM lane) and 32 of a tile's 64 query columns, so the
+//              sum over queries is thread-local and the two halves meet once at the end,
+//   warp 8     TMA producer of the Q, C and position tiles; its lanes also bring the tile's lse values,
+//   warp 9     UMMA issuer and TMEM owner.
+// Per tile S^T = K Q^T (M128 N64 K64) and U^T = B~ C^T (K32) land in one of two TMEM buffers, so the next
+// tile's GEMMs run under this tile's arithmetic; two CTAs share an SM (2 x 256 TMEM columns).
+// Off the diagonal the decay is the product of three factors <= 1: the query's within its 64-row block (a
+// stored plane), the one between the blocks (one per tile) and the key's to the end of its tile (one per
+// thread). F_i - F_j is taken before the log2e scaling. Per element that leaves 3 packed-fp32 issue slots
+// and one exponential.
+// Sums: a tile's 32 shares are added in two packed chains and then join the running sum, so a sum over
+// 16384 queries is a chain of 256 additions and not of 16384.
 #include <cuda_runtime.h>
-#include <cstdint>
 
-#include "sm100.cuh"
+#include "attn_common.cuh"
 #include "key_weights.h"
 
 namespace sisa {
 namespace kwt {
 
-constexpr int NT = 128, QT = 32;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int BK = 128, BQ = 64, NSTAGE = 4, NCW = 8;            // keys, queries per tile, stages, compute warps
+constexpr uint32_t SZ_K = BK * 128, SZ_B = BK * 64;
+constexpr uint32_t SZ_Q = BQ * 128, SZ_C = BQ * 64, SZ_POS = BQ * 16, SZ_LSE = BQ * 4;
+constexpr uint32_t OFFS_C = SZ_Q, OFFS_POS = OFFS_C + SZ_C, OFFS_LSE = OFFS_POS + SZ_POS;
+constexpr uint32_t SZ_STAGE = 14 * 1024;
+static_assert(OFFS_LSE + SZ_LSE <= SZ_STAGE, "stage");
+constexpr uint32_t OFF_K = 0, OFF_B = OFF_K + SZ_K, OFF_ST = OFF_B + SZ_B;
+constexpr uint32_t OFF_SUM = OFF_ST + NSTAGE * SZ_STAGE, OFF_BAR = OFF_SUM + BK * 4;
+constexpr uint32_t SMEM_BYTES = OFF_BAR + 256 + 1024;
+static_assert(OFF_ST % 1024 == 0 && SZ_STAGE % 1024 == 0, "swizzle alignment");
+static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
+constexpr uint32_t TMEM_COLS = 256;                              // two buffers of S^T (64) and U^T (64)
+constexpr int B_K = 0, B_QF = 1, B_QE = B_QF + NSTAGE, B_SF = B_QE + NSTAGE, B_SE = B_SF + 2;
+static_assert((B_SE + 2) * 8 <= 128, "barriers end below the TMEM slot");
+constexpr int NT = (NCW + 2) * 32;
 
 template <bool kHalf>
-__global__ void __launch_bounds__(NT) key_weights_kernel(KeyWeightParams p) {
-  __shared__ float s_q[QT][64], s_c[QT][32], s_g[QT], s_a[QT];
-  const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H, tid = threadIdx.x;
-  const int k0 = blockIdx.x * NT, j = k0 + tid;
-  const bool ok = j < p.L;
-  float kr[64], br[32];
-  const uint4* kp = reinterpret_cast<const uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + (int64_t)(ok ? j : 0) * p.k_sl));
-  const uint4* bp = reinterpret_cast<const uint4*>(p.b + 2 * (b * p.b_sb + h * p.b_sh + (int64_t)(ok ? j : 0) * p.b_sl));
-#pragma unroll
-  for (int i = 0; i < 12; ++i) {
-    const uint4 v = i < 8 ? kp[i] : bp[i - 8];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float* d = i < 8 ? kr + 8 * i : br + 8 * (i - 8);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { d[2 * e] = unpack_lo<kHalf>(w[e]); d[2 * e + 1] = unpack_hi<kHalf>(w[e]); }
+__global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constant__ KeyWeightParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int bh, kt;
+  tile_order(p.ntk, p.B * p.H, bh, kt);            // the first key tiles have the most queries
+  const int b = bh / p.H, h = bh % p.H;
+  const int L = p.L, k0 = kt * BK;
+  const int i_begin = max(p.first, k0) / BQ * BQ;
+  const int ntiles = (L - i_begin + BQ - 1) / BQ;  // >= 1: k0 < L and first < L
+
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (sbase - raw);
+  const uint32_t sK = sbase + OFF_K, sB = sbase + OFF_B;
+  const uint32_t bar0 = sbase + OFF_BAR;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + OFF_BAR + 128);
+#define BAR(i) (bar0 + 8u * (uint32_t)(i))
+  auto stage_addr = [&](int s) { return sbase + OFF_ST + (uint32_t)s * SZ_STAGE; };
+
+  if (tid == 0) {
+    mbar_init(BAR(B_K), 1);
+    for (int s = 0; s < NSTAGE; ++s) {
+      mbar_init(BAR(B_QF + s), 33);                // the TMA bytes and 32 lanes' lse values
+      mbar_init(BAR(B_QE + s), NCW + 1);           // the compute warps and the UMMAs
+    }
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(BAR(B_SF + u), 1);
+      mbar_init(BAR(B_SE + u), NCW);
+    }
+    fence_barrier_init();
   }
-  const float* pos = p.pos + (int64_t)bh * 4 * p.Lp;
-  const float gj = ok ? pos[j] : 0.f, fj = ok ? pos[p.Lp + j] : 0.f;
-  const float lam = p.lam[h];
-  float acc = 0.f;
-  for (int i0 = max(p.first, k0) / QT * QT; i0 < p.L; i0 += QT) {
-    __syncthreads();
-    for (int e = tid; e < QT * 96; e += NT) {
-      const int r = e / 96, d = e % 96, i = i0 + r;
-      float x = 0.f;
-      if (i < p.L) {
-        const char* src = d < 64 ? p.q + 2 * (b * p.q_sb + h * p.q_sh + i * p.q_sl + d)
-                                 : p.c + 2 * (b * p.c_sb + h * p.c_sh + i * p.c_sl + d - 64);
-        x = unpack_lo<kHalf>(*reinterpret_cast<const uint16_t*>(src));
+  if (warp == NCW + 1) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+
+  if (warp == NCW) {
+    // ------------------------------------------------------------------ producer
+    if (lane == 0) {
+      mbar_expect_tx(BAR(B_K), SZ_K + SZ_B);
+      tma_load_4d(sK, &p.tm_k, BAR(B_K), 0, k0, h, b);
+      tma_load_4d(sB, &p.tm_b, BAR(B_K), 0, k0, h, b);
+    }
+    const float* lse = p.lse + (int64_t)bh * L;
+    auto lse_at = [&](int i) { return i < L ? -__ldg(lse + i) : 0.f; };
+    float n0 = lse_at(i_begin + lane), n1 = lse_at(i_begin + lane + 32);
+    for (int n = 0; n < ntiles; ++n) {
+      const int s = n % NSTAGE, i0 = i_begin + n * BQ;
+      if (n >= NSTAGE && !warp_wait<true>(BAR(B_QE + s), ((n / NSTAGE) - 1) & 1, p.status)) break;
+      const uint32_t st = stage_addr(s);
+      if (lane == 0) {
+        mbar_expect_tx(BAR(B_QF + s), SZ_Q + SZ_C + SZ_POS);
+        tma_load_4d(st, &p.tm_q, BAR(B_QF + s), 0, i0, h, b);
+        tma_load_4d(st + OFFS_C, &p.tm_c, BAR(B_QF + s), 0, i0, h, b);
+        tma_load_3d(st + OFFS_POS, &p.tm_pos, BAR(B_QF + s), i0, 0, bh);
       }
-      if (d < 64) s_q[r][d] = x; else s_c[r][d - 64] = x;
+      float* nl = reinterpret_cast<float*>(gbase + OFF_ST + s * SZ_STAGE + OFFS_LSE);
+      nl[lane] = n0;                               // -lse of this tile's queries
+      nl[lane + 32] = n1;
+      mbar_arrive(BAR(B_QF + s));
+      n0 = lse_at(i0 + BQ + lane);                 // the next tile's, in flight while this warp waits
+      n1 = lse_at(i0 + BQ + lane + 32);
     }
-    if (tid < QT && i0 + tid < p.L) {
-      s_g[tid] = pos[i0 + tid];
-      s_a[tid] = p.lse[(int64_t)bh * p.L + i0 + tid];
+  } else if (warp == NCW + 1) {
+    // ------------------------------------------------------------------ UMMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc(128, 64, kHalf ? 0 : 1, 0, 0);
+      bool ok = mbar_wait<true>(BAR(B_K), 0, p.status);
+      for (int n = 0; ok && n < ntiles; ++n) {
+        const int s = n % NSTAGE, u = n & 1;
+        if (!mbar_wait<true>(BAR(B_QF + s), (n / NSTAGE) & 1, p.status)) break;
+        if (n >= 2 && !mbar_wait<true>(BAR(B_SE + u), ((n >> 1) - 1) & 1, p.status)) break;
+        tc_fence_after();
+        const uint32_t st = stage_addr(s), tS = tbase + u * 128, tU = tS + 64;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_ss(tS, desc_k128(sK + k * 32), desc_k128(st + k * 32), idesc, k > 0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          umma_ss(tU, desc_k64(sB + k * 32), desc_k64(st + OFFS_C + k * 32), idesc, k > 0);
+        umma_commit(BAR(B_SF + u));
+        umma_commit(BAR(B_QE + s));
+      }
     }
-    __syncthreads();
-    const int hi = min(QT, p.L - i0);
-    for (int r = 0; r < hi; ++r) {
-      const int i = i0 + r;
-      if (!ok || i < j || i < p.first) continue;
-      float qk = 0.f, cb = 0.f;
+  } else {
+    // ------------------------------------------------------------------ compute
+    const int r = tid & 127, half = warp >> 2;     // key row of the tile, which 32 query columns
+    const int j = k0 + r;
+    const float* posbh = p.pos + (int64_t)bh * 4 * p.Lp;
+    const int jj = min(j, L - 1), je = min(k0 + BK, L) - 1;
+    const float gj = posbh[jj], fj = posbh[p.Lp + jj], gend = posbh[je];
+    const float lam2 = p.lam[h] * kLOG2E;
+    const float cj = lam2 * exp2f(fmin_nan((gend - gj) * kLOG2E, 0.f));
+    const float2 nfj = bcast2(-fj), l2e = bcast2(kLOG2E), c1 = bcast2(kScale * kLOG2E);
+    float2 total = bcast2(0.f);
+    bool ok = true;
+    for (int n = 0; n < ntiles; ++n) {
+      const int s = n % NSTAGE, u = n & 1, i0 = i_begin + n * BQ;
+      // the scores, and the lse values that the producer's lanes stored
+      if (!warp_wait_tested<true>(BAR(B_SF + u), (n >> 1) & 1, p.status) ||
+          !warp_wait_tested<true>(BAR(B_QF + s), (n / NSTAGE) & 1, p.status)) { ok = false; break; }
+      tc_fence_after();
+      float sv[32], uv[32];
+      tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + half * 32), sv);
+      tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + 64 + half * 32), uv);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(B_SE + u));   // the buffer may take the tile after next
+      const float* q = reinterpret_cast<const float*>(gbase + OFF_ST + s * SZ_STAGE + OFFS_POS);
+      const float4* qf4 = reinterpret_cast<const float4*>(q + BQ) + half * 8;           // F_i
+      const float4* qr4 = reinterpret_cast<const float4*>(q + 2 * BQ) + half * 8;       // decay within the block
+      const float4* ql4 = reinterpret_cast<const float4*>(q + 4 * BQ) + half * 8;       // -lse_i
+      float2 t0 = bcast2(0.f), t1 = bcast2(0.f);
+      if (i0 >= k0 + BK && i0 >= p.first && i0 + BQ <= L) {
+        const float2 cm = bcast2(cj * exp2f(fmin_nan((q[0] - gend) * kLOG2E, 0.f)));
 #pragma unroll
-      for (int d = 0; d < 64; ++d) qk = fmaf(s_q[r][d], kr[d], qk);
+        for (int c = 0; c < 8; ++c) {
+          const float4 f4 = qf4[c], r4 = qr4[c], l4 = ql4[c];
 #pragma unroll
-      for (int d = 0; d < 32; ++d) cb = fmaf(s_c[r][d], br[d], cb);
-      const float dec = exp2f(fmin_nan((s_g[r] - gj) * kLog2e, 0.f));
-      const float s = fmaf(qk, 0.125f, lam * (dec * cb)) + (pos[p.Lp + i] - fj);
-      acc += exp2f(fmaf(s, kLog2e, -s_a[r]));
+          for (int e = 0; e < 2; ++e) {
+            const float2 fi = e ? make_float2(f4.z, f4.w) : make_float2(f4.x, f4.y);
+            const float2 rf = e ? make_float2(r4.z, r4.w) : make_float2(r4.x, r4.y);
+            const float2 nl = e ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+            const int at = 4 * c + 2 * e;
+            const float2 y = fma2(add2(fi, nfj), l2e, nl);
+            const float2 d = fma2(mul2(make_float2(uv[at], uv[at + 1]), rf), cm, y);
+            const float2 x = fma2(make_float2(sv[at], sv[at + 1]), c1, d);
+            const float2 pe = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            if (e) t1 = add2(t1, pe); else t0 = add2(t0, pe);
+          }
+        }
+      } else {
+        // tiles on the diagonal, at `first` or at the end: pairwise decay, masked shares
+        const float* qg = q + half * 32;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const int i = i0 + half * 32 + c;
+          const float dec = exp2f(fmin_nan((qg[c] - gj) * kLOG2E, 0.f));
+          const float y = fmaf(qg[BQ + c] - fj, kLOG2E, qg[4 * BQ + c]);
+          const float x = fmaf(sv[c], kScale * kLOG2E, fmaf(uv[c] * dec, lam2, y));
+          const float pe = (i >= j && i >= p.first && i < L) ? ex2_approx(x) : 0.f;
+          if (c & 1) t0.y += pe; else t0.x += pe;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(B_QE + s));
+      total = add2(total, add2(t0, t1));
+    }
+    float* sums = reinterpret_cast<float*>(gbase + OFF_SUM);
+    const float mine = total.x + total.y;
+    if (half) sums[r] = mine;
+    named_bar_sync(1, NCW * 32);
+    if (!half && j < L) {
+      const float w = mine + sums[r];
+      p.w[(int64_t)bh * L + j] = w;
+      if (ok && !isfinite(w) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
     }
   }
-  if (ok) p.w[(int64_t)bh * p.L + j] = acc;
-  if (ok && !isfinite(acc) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NCW + 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, TMEM_COLS);
+  }
+#undef BAR
 }
 
 }  // namespace kwt
 
 cudaError_t launch_key_weights(const KeyWeightParams& p, int dtype, cudaStream_t st) {
-  dim3 grid((p.L + kwt::NT - 1) / kwt::NT, p.B * p.H);
-  if (dtype == 1) kwt::key_weights_kernel<true><<<grid, kwt::NT, 0, st>>>(p);
-  else kwt::key_weights_kernel<false><<<grid, kwt::NT, 0, st>>>(p);
+  using namespace kwt;
+  dim3 grid(p.ntk, p.B * p.H);
+  if (dtype == 1) {
+    cudaFuncSetAttribute(key_weights_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    key_weights_kernel<true><<<grid, NT, SMEM_BYTES, st>>>(p);
+  } else {
+    cudaFuncSetAttribute(key_weights_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    key_weights_kernel<false><<<grid, NT, SMEM_BYTES, st>>>(p);
+  }
   return cudaGetLastError();
 }
 
