@@ -30,8 +30,9 @@ struct PagedAttnParams {
   char* y; int64_t y_sb, y_sh;           // (B, H, 1, 64) low precision
   float* lse;                            // (B, H) log2 units, or null
   float* weight_out;                     // null: weights are not accumulated
-  float* ws;                             // partial records, then the scores with weight_out
-  int B, H, splits;
+  float* ws;                             // the workspace; its parts are set by launch_paged_attn:
+  float* records; float* lse_all; float* scores;
+  int B, H;
   int64_t max_keys;                      // max_pages << page_shift
   int32_t* status;
 };
@@ -75,8 +76,8 @@ struct PagedFillParams {
   int32_t* status;
 };
 
-int paged_attn_splits(int64_t B, int64_t H, int64_t max_keys);
-cudaError_t launch_paged_attn(const PagedAttnParams& p, int dtype, cudaStream_t st);
+int64_t paged_attn_workspace_floats(int64_t units, int64_t max_keys, bool scores);
+cudaError_t launch_paged_attn(PagedAttnParams p, int dtype, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictParams& p, cudaStream_t st);
 cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, cudaStream_t st);
 cudaError_t launch_paged_fill(const PagedFillParams& p, cudaStream_t st);

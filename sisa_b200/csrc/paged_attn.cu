@@ -1,192 +1,478 @@
-// paged_attn.cu - attention of one new token per sequence over its paged keys.
+// paged_attn.cu - attention of one new token per sequence over its paged keys, split over the keys and joined.
 //
 // For every sequence b with n_b keys (slots 0 .. n_b - 1 of its pages, in any order) and head h:
 //   x_j = log2e (q.k_j / 8 + lam_h exp(min(g_q - g_j, 0)) (c.b~_j) + (F_q - F_j)),
 //   y = sum_j 2^(x_j - lse) v_j,  lse = log2 sum_j 2^x_j,  and optionally weight_j += 2^(x_j - lse).
 // A row with no keys gives y = 0 and lse = -inf.
+//
+// HBM-bound: 328 bytes per key and head (k, v, b~ in 16 bits, g and F in 32), 320 flops. Work is cut into
+// tiles of 32 keys; the tiles of all (sequence, head) units lie in one line, and each of a fixed number of
+// warps takes an equal run of it, so sequences of any mix of lengths load every SM alike. A warp is on its
+// own: it fills a ring of stages in shared memory by bulk copies (one lane per operand, rows of a page are
+// dense), reads each tile once, keeps the running maximum (moved only when a key exceeds it by 2^8), the
+// sum and the 64 output sums in registers, and never meets a block-wide barrier. Eight lanes share a key
+// (16 bytes of its rows each), so a tile is eight groups of four keys; the eight partial dot products of a
+// lane are summed by a reduce-scatter over the eight lanes, after which every lane owns one key's score and
+// the exponentials are taken once per key.
+// A unit inside one warp's run is finished there; the others leave (m, l, acc) records, at most two per
+// warp, that paged_join_kernel merges in warp order (deterministic, no atomics). With weights, the scores
+// are kept in the workspace (4 bytes per key) and paged_weights_kernel adds the shares once lse is known.
 #include <cuda_runtime.h>
 #include <cstdint>
 
-#include "sm100.cuh"
+#include "attn_common.cuh"
 #include "paged.h"
 
 namespace sisa {
 namespace pat {
 
-constexpr int NT = 256, NW = NT / 32;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int TK = 32;                          // keys per tile
+constexpr int NW = 4, NSTAGE = 5;               // warps per CTA, ring stages per warp
+constexpr int NCTA = 148, NWORK = NCTA * NW;    // one CTA per SM
+constexpr uint32_t OFF_V = TK * 128, OFF_B = OFF_V + TK * 128, OFF_G = OFF_B + TK * 64, OFF_F = OFF_G + TK * 4;
+constexpr uint32_t SZ_STAGE = OFF_F + TK * 4;   // 10,496 bytes
+constexpr uint32_t SZ_WARP = NSTAGE * SZ_STAGE;
+constexpr uint32_t OFF_BAR = NW * SZ_WARP, OFF_MASK = OFF_BAR + NW * NSTAGE * 8;
+constexpr uint32_t SMEM_BYTES = OFF_MASK + NW * NSTAGE * 4 + 128;
+static_assert(SZ_STAGE % 128 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory");
+constexpr int REC = 68;                         // floats of a record: m, l, 2 unused, acc[64]
 
-template <bool kHalf>
-__device__ __forceinline__ void unpack8(const uint4& v, float* out) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ int64_t keys_of(const PagedAttnParams& p, int b) {
+  const int64_t n = __ldg(p.lengths + b);
+  return n < 0 ? 0 : (n > p.max_keys ? p.max_keys : n);
+}
+__device__ __forceinline__ int64_t tiles_of(const PagedAttnParams& p, int b) { return (keys_of(p, b) + TK - 1) / TK; }
+
+// Tiles per head of the sequences before b (all of them with b = B), computed by one warp.
+__device__ __forceinline__ int64_t tiles_before(const PagedAttnParams& p, int b, int64_t& all) {
+  int64_t before = 0, total = 0;
+  for (int i = threadIdx.x & 31; i < p.B; i += 32) {
+    const int64_t t = tiles_of(p, i);
+    total += t;
+    if (i < b) before += t;
+  }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    out[2 * e] = unpack_lo<kHalf>(w[e]);
-    out[2 * e + 1] = unpack_hi<kHalf>(w[e]);
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  all = total;
+  return before;
+}
+
+// The line is shared by min(NWORK, tiles) workers, so none of them has an empty run: worker w takes the tiles
+// [run_start(w), run_start(w + 1)); worker_of is its inverse.
+__device__ __forceinline__ int64_t workers(int64_t tiles) { return tiles < NWORK ? tiles : NWORK; }
+__device__ __forceinline__ int64_t run_start(int64_t w, int64_t tiles) { return w * tiles / workers(tiles); }
+__device__ __forceinline__ int worker_of(int64_t x, int64_t tiles) {
+  return (int)(((x + 1) * workers(tiles) - 1) / tiles);
+}
+
+// A place in the line: tile t of the T tiles of (b, h).
+struct Cursor {
+  int b, h;
+  int64_t t, T, n;
+  __device__ __forceinline__ void load(const PagedAttnParams& p) { n = keys_of(p, b); T = (n + TK - 1) / TK; }
+  // The next tile of the line (the caller knows that there is one).
+  __device__ __forceinline__ void next(const PagedAttnParams& p) {
+    if (++t < T) return;
+    t = 0;
+    if (++h < p.H) return;
+    h = 0;
+    do { ++b; load(p); } while (T == 0);
+  }
+};
+
+// The cursor of tile x, found by one warp.
+__device__ __forceinline__ Cursor find_tile(const PagedAttnParams& p, int64_t x) {
+  const int lane = threadIdx.x & 31;
+  int64_t base = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int64_t t = b0 + lane < p.B ? tiles_of(p, b0 + lane) : 0;
+    int64_t incl = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const int64_t lo = (base + incl - t) * p.H;
+    const uint32_t hit = __ballot_sync(0xffffffffu, t > 0 && x >= lo && x < lo + t * p.H);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int64_t T = __shfl_sync(0xffffffffu, t, src), rem = x - __shfl_sync(0xffffffffu, lo, src);
+      Cursor c;
+      c.b = b0 + src;
+      c.h = (int)(rem / T);
+      c.t = rem - c.h * T;
+      c.load(p);
+      return c;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
   }
 }
 
-__device__ __forceinline__ int64_t keys_of(const PagedAttnParams& p, int b) {
-  const int64_t n = p.lengths[b];
-  return n < 0 ? 0 : (n > p.max_keys ? p.max_keys : n);
+template <bool kHalf>
+__device__ __forceinline__ float2 unpack2(uint32_t w) { return make_float2(unpack_lo<kHalf>(w), unpack_hi<kHalf>(w)); }
+
+// Eight values per lane summed over the eight lanes of a key group: lane `part` gets the sum of value part.
+__device__ __forceinline__ float reduce_scatter8(const float (&v)[8], int part) {
+  float a[4], c[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool hi = part & 4;
+    a[i] = (hi ? v[i + 4] : v[i]) + __shfl_xor_sync(0xffffffffu, hi ? v[i] : v[i + 4], 4);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool hi = part & 2;
+    c[i] = (hi ? a[i + 2] : a[i]) + __shfl_xor_sync(0xffffffffu, hi ? a[i] : a[i + 2], 2);
+  }
+  const bool hi = part & 1;
+  return (hi ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, hi ? c[0] : c[1], 1);
 }
 
-// Grid (splits, B*H). Eight lanes per key, each with 16 bytes of the key's k, v and b~ rows; every warp
-// runs its own online softmax over groups of four keys, merged once at the end.
-template <bool kHalf>
-__global__ void __launch_bounds__(NT) paged_split_kernel(PagedAttnParams p) {
-  const int split = blockIdx.x, bh = blockIdx.y;
-  const int b = bh / p.H, h = bh % p.H;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t N = keys_of(p, b);
-  if (split == 0 && h == 0 && tid == 0 && p.lengths[b] > p.max_keys && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
-  const int64_t per = (N + p.splits - 1) / p.splits;
-  const int64_t j_begin = split * per, j_end = min(N, j_begin + per);
-  __shared__ float s_m[NW], s_l[NW];
-  __shared__ float s_acc[NW][64];
-  const int sub = lane >> 3, part = lane & 7;
-  float q8[8], c8[8];
-  unpack8<kHalf>(reinterpret_cast<const uint4*>(p.q + 2 * ((int64_t)b * p.q_sb + (int64_t)h * p.q_sh))[part], q8);
-  uint4 cv = make_uint4(0, 0, 0, 0);
-  if (part < 4) cv = reinterpret_cast<const uint4*>(p.c + 2 * ((int64_t)b * p.c_sb + (int64_t)h * p.c_sh))[part];
-  unpack8<kHalf>(cv, c8);
-  const float gq = p.g_q[bh], fq = p.f_q ? p.f_q[bh] : 0.f;
-  const float c1 = 0.125f * kLog2e, lam2 = p.lam[h] * kLog2e;
-  float* xs = p.weight_out ? p.ws + (int64_t)p.splits * p.B * p.H * 66 + (int64_t)bh * p.max_keys : nullptr;
-  float m_ref = -INFINITY, lsum = 0.f, acc[8];
-#pragma unroll
-  for (int d = 0; d < 8; ++d) acc[d] = 0.f;
-#pragma unroll 1
-  for (int64_t j0 = j_begin + 4 * warp; j0 < j_end; j0 += 4 * NW) {
-    const int64_t j = j0 + sub;
-    const int page = j < j_end ? page_of(p.pg, b, j, p.status) : -1;
-    const bool ok = page >= 0;
-    uint4 kv = make_uint4(0, 0, 0, 0), vv = kv, bv = kv;
-    float gj = 0.f, fj = 0.f;
-    if (ok) {
-      const int64_t slot = j & ((1 << p.pg.page_shift) - 1);
-      kv = reinterpret_cast<const uint4*>(p.pg.k + 2 * (page * p.pg.k_sp + h * p.pg.k_sh + slot * 64))[part];
-      vv = reinterpret_cast<const uint4*>(p.pg.v + 2 * (page * p.pg.v_sp + h * p.pg.v_sh + slot * 64))[part];
-      if (part < 4) bv = reinterpret_cast<const uint4*>(p.pg.b + 2 * (page * p.pg.b_sp + h * p.pg.b_sh + slot * 32))[part];
-      gj = p.pg.g[page * p.pg.s_sp + h * p.pg.s_sh + slot];
-      if (p.f_q) fj = p.pg.f[page * p.pg.s_sp + h * p.pg.s_sh + slot];
+template <bool kHalf, bool kScores>
+__global__ void __launch_bounds__(NW * 32, 1) paged_attn_kernel(PagedAttnParams p) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t raw = smem_u32(smem_raw), sbase = (raw + 127u) & ~127u;
+  uint8_t* gbase = smem_raw + (sbase - raw);
+  const uint32_t ring = sbase + warp * SZ_WARP, bars = sbase + OFF_BAR + warp * NSTAGE * 8;
+  uint8_t* gring = gbase + warp * SZ_WARP;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(gbase + OFF_MASK) + warp * NSTAGE;
+  if (lane == 0) {
+    for (int s = 0; s < NSTAGE; ++s) mbar_init(bars + 8 * s, 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+
+  int64_t per_head;
+  tiles_before(p, 0, per_head);
+  const int64_t tiles = per_head * p.H;
+  const int w = blockIdx.x + NCTA * warp;       // a short line is spread over the SMs first
+  if (w == 0) {                                 // lengths past the table, once per sequence
+    for (int b = lane; b < p.B; b += 32)
+      if (__ldg(p.lengths + b) > p.max_keys && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
+  }
+  if (w >= workers(tiles)) return;
+  const int64_t x0 = run_start(w, tiles), count = run_start(w + 1, tiles) - x0;
+
+  // ---- this lane's part of a tile's copies: operand op of the tile's sub-tile sub (pages of 16 slots
+  // give a tile two sub-tiles)
+  const int op = lane & 7, sub = lane >> 3;
+  const int nsub = p.pg.page_shift < 5 ? 2 : 1, rows_max = p.pg.page_shift < 5 ? 16 : TK;
+  const char* src0 = nullptr;
+  int64_t src_p = 0, src_h = 0;                 // page and head strides in bytes
+  int row_bytes = 0;
+  uint32_t dst_off = 0;
+  if (op == 0) { src0 = p.pg.k; src_p = p.pg.k_sp * 2; src_h = p.pg.k_sh * 2; row_bytes = 128; }
+  if (op == 1) { src0 = p.pg.v; src_p = p.pg.v_sp * 2; src_h = p.pg.v_sh * 2; row_bytes = 128; dst_off = OFF_V; }
+  if (op == 2) { src0 = p.pg.b; src_p = p.pg.b_sp * 2; src_h = p.pg.b_sh * 2; row_bytes = 64; dst_off = OFF_B; }
+  if (op == 3) { src0 = (const char*)p.pg.g; src_p = p.pg.s_sp * 4; src_h = p.pg.s_sh * 4; row_bytes = 4; dst_off = OFF_G; }
+  if (op == 4 && p.f_q) { src0 = (const char*)p.pg.f; src_p = p.pg.s_sp * 4; src_h = p.pg.s_sh * 4; row_bytes = 4; dst_off = OFF_F; }
+  dst_off += sub * rows_max * row_bytes;
+  const bool copier = sub < nsub && row_bytes > 0;
+  const uint32_t key_bytes = 128 + 128 + 64 + 4 + (p.f_q ? 4 : 0);
+
+  Cursor in = find_tile(p, x0), at = in;
+  // the page of this lane's sub-tile at the fill cursor, read one tile ahead of its use
+  auto page_at = [&]() {
+    const int64_t j = in.t * TK + sub * rows_max;
+    return sub < nsub && j < in.n ? __ldg(p.pg.table + (int64_t)in.b * p.pg.table_sb + (j >> p.pg.page_shift)) : -1;
+  };
+  int page = page_at();
+  int64_t filled = 0;
+  auto fill = [&](int s) {
+    const int64_t j = in.t * TK + sub * rows_max;
+    const int left = (int)(in.n - j < rows_max ? in.n - j : rows_max);       // keys of this sub-tile
+    const bool used = sub < nsub && left > 0;
+    const bool good = used && (unsigned)page < (unsigned)p.pg.n_pages;
+    if (used && !good && op == 0 && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
+    const int rows = good ? (left + 3) & ~3 : 0;                             // copies are whole 16-byte units
+    const uint32_t bits = good ? (left >= 32 ? 0xffffffffu : (1u << left) - 1) << (sub * rows_max) : 0u;
+    const int rows1 = __shfl_sync(0xffffffffu, rows, 8);
+    const uint32_t bits1 = __shfl_sync(0xffffffffu, bits, 8);
+    if (lane == 0) {
+      masks[s] = bits | bits1;
+      mbar_expect_tx(bars + 8 * s, (uint32_t)(rows + rows1) * key_bytes);
     }
-    float k8[8], b8[8], v8[8];
-    unpack8<kHalf>(kv, k8);
-    unpack8<kHalf>(bv, b8);
-    unpack8<kHalf>(vv, v8);
-    float qk = 0.f, cb = 0.f;
+    __syncwarp();
+    if (copier && rows > 0)
+      bulk_load(ring + s * SZ_STAGE + dst_off,
+                src0 + page * src_p + in.h * src_h + (j & ((1 << p.pg.page_shift) - 1)) * row_bytes,
+                (uint32_t)(rows * row_bytes), bars + 8 * s);
+    ++filled;
+    if (filled < count) {
+      in.next(p);
+      page = page_at();
+    }
+  };
+  for (int s = 0; s < NSTAGE && filled < count; ++s) fill(s);
+
+  const int quad = lane >> 3, part = lane & 7;  // a lane holds 16 bytes (part) of key quad of every group
+  const int key = 4 * part + quad;              // the key whose score this lane ends up with
+  const float c1 = kScale * kLOG2E;
+  float2 q2[4], c2[2], acc[4];
+  float gq = 0.f, fq = 0.f, lam2 = 0.f, m_ref = -INFINITY, lsum = 0.f;
+  int64_t seg = 0;                              // tiles of the unit done in this run
+  bool ok = true;
+#pragma unroll 1
+  for (int64_t i = 0; i < count; ++i) {
+    if (seg == 0) {                             // a new unit: its query row and constants
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.q + 2 * (at.b * p.q_sb + at.h * p.q_sh)) + part);
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.c + 2 * (at.b * p.c_sb + at.h * p.c_sh)) + part);
+      q2[0] = unpack2<kHalf>(v.x); q2[1] = unpack2<kHalf>(v.y); q2[2] = unpack2<kHalf>(v.z); q2[3] = unpack2<kHalf>(v.w);
+      c2[0] = unpack2<kHalf>(u.x); c2[1] = unpack2<kHalf>(u.y);
+      const int64_t bh = (int64_t)at.b * p.H + at.h;
+      gq = __ldg(p.g_q + bh);
+      fq = p.f_q ? __ldg(p.f_q + bh) : 0.f;
+      lam2 = __ldg(p.lam + at.h) * kLOG2E;
+      m_ref = -INFINITY;
+      lsum = 0.f;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) acc[d] = bcast2(0.f);
+    }
+    const int s = (int)(i % NSTAGE);
+    if (!warp_wait_tested<true>(bars + 8 * s, (uint32_t)(i / NSTAGE) & 1, p.status)) { ok = false; break; }
+    const uint8_t* st = gring + s * SZ_STAGE;
+    const uint32_t mask = masks[s];
+    float qk[8], cb[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      qk = fmaf(q8[e], k8[e], qk);
-      cb = fmaf(c8[e], b8[e], cb);
+      const uint4 kv = reinterpret_cast<const uint4*>(st)[e * 32 + lane];
+      const uint2 bv = reinterpret_cast<const uint2*>(st + OFF_B)[e * 32 + lane];
+      float2 a = mul2(q2[0], unpack2<kHalf>(kv.x)), d = mul2(c2[0], unpack2<kHalf>(bv.x));
+      a = fma2(q2[1], unpack2<kHalf>(kv.y), a);
+      a = fma2(q2[2], unpack2<kHalf>(kv.z), a);
+      a = fma2(q2[3], unpack2<kHalf>(kv.w), a);
+      d = fma2(c2[1], unpack2<kHalf>(bv.y), d);
+      qk[e] = a.x + a.y;
+      cb[e] = d.x + d.y;
     }
-    const float dec = exp2f(fmin_nan((gq - gj) * kLog2e, 0.f));
-    float x = fmaf(qk, c1, lam2 * (dec * cb));
-    x += __shfl_xor_sync(0xffffffffu, x, 1);
-    x += __shfl_xor_sync(0xffffffffu, x, 2);
-    x += __shfl_xor_sync(0xffffffffu, x, 4);
-    x = ok ? fmaf(fq - fj, kLog2e, x) : -INFINITY;
-    if (xs && part == 0 && j < j_end) xs[j] = x;
-    float mx = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-    if (mx > m_ref + 8.f) {
+    const float gj = reinterpret_cast<const float*>(st + OFF_G)[key];
+    const float fj = p.f_q ? reinterpret_cast<const float*>(st + OFF_F)[key] : 0.f;
+    const float dec = exp2f(fmin_nan((gq - gj) * kLOG2E, 0.f));
+    float x = fmaf(reduce_scatter8(qk, part), c1, lam2 * (dec * reduce_scatter8(cb, part)));
+    x = (mask >> key) & 1 ? fmaf(fq - fj, kLOG2E, x) : -INFINITY;
+    if constexpr (kScores) {
+      if (at.t * TK + key < at.n) p.scores[((int64_t)at.b * p.H + at.h) * p.max_keys + at.t * TK + key] = x;
+    }
+    if (__any_sync(0xffffffffu, x > m_ref + 8.f)) {
+      float mx = x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       const float corr = (m_ref == -INFINITY) ? 0.f : exp2f(m_ref - mx);
 #pragma unroll
-      for (int d = 0; d < 8; ++d) acc[d] *= corr;
+      for (int d = 0; d < 4; ++d) acc[d] = mul2(acc[d], bcast2(corr));
       lsum *= corr;
       m_ref = mx;
     }
-    const float pj = ok ? exp2f(x - (m_ref == -INFINITY ? 0.f : m_ref)) : 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = fmaf(pj, v8[e], acc[e]);
+    const float pj = exp2f(x - (m_ref == -INFINITY ? 0.f : m_ref));
     lsum += pj;
+    if (mask == 0xffffffffu) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 pe = bcast2(__shfl_sync(0xffffffffu, pj, (lane & 24) + e));
+        const uint4 v = reinterpret_cast<const uint4*>(st + OFF_V)[e * 32 + lane];
+        acc[0] = fma2(pe, unpack2<kHalf>(v.x), acc[0]);
+        acc[1] = fma2(pe, unpack2<kHalf>(v.y), acc[1]);
+        acc[2] = fma2(pe, unpack2<kHalf>(v.z), acc[2]);
+        acc[3] = fma2(pe, unpack2<kHalf>(v.w), acc[3]);
+      }
+    } else {
+      // a partial tile: whatever lies in the slots past the end (NaN too) must not meet the sums
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        const float2 pe = bcast2(__shfl_sync(0xffffffffu, pj, (lane & 24) + e));
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if ((mask >> (4 * e + quad)) & 1) v = reinterpret_cast<const uint4*>(st + OFF_V)[e * 32 + lane];
+        acc[0] = fma2(pe, unpack2<kHalf>(v.x), acc[0]);
+        acc[1] = fma2(pe, unpack2<kHalf>(v.y), acc[1]);
+        acc[2] = fma2(pe, unpack2<kHalf>(v.z), acc[2]);
+        acc[3] = fma2(pe, unpack2<kHalf>(v.w), acc[3]);
+      }
+    }
+    __syncwarp();                               // every lane has read the stage
+    if (filled < count) fill(s);
+    ++seg;
+    if (at.t + 1 == at.T || i + 1 == count) {
+      // ---- the unit ends here, or the run does: this run's m, l and 64 sums
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        acc[d].x += __shfl_xor_sync(0xffffffffu, acc[d].x, 8);
+        acc[d].y += __shfl_xor_sync(0xffffffffu, acc[d].y, 8);
+        acc[d].x += __shfl_xor_sync(0xffffffffu, acc[d].x, 16);
+        acc[d].y += __shfl_xor_sync(0xffffffffu, acc[d].y, 16);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+      const int64_t bh = (int64_t)at.b * p.H + at.h;
+      if (seg == at.T) {                        // the whole unit
+        const float lse = m_ref + log2f(lsum), r = 1.f / lsum;
+        if (quad == 0) {
+          const uint4 o = make_uint4(pack2<kHalf>(acc[0].x * r, acc[0].y * r), pack2<kHalf>(acc[1].x * r, acc[1].y * r),
+                                     pack2<kHalf>(acc[2].x * r, acc[2].y * r), pack2<kHalf>(acc[3].x * r, acc[3].y * r));
+          reinterpret_cast<uint4*>(p.y + 2 * (at.b * p.y_sb + at.h * p.y_sh))[part] = o;
+        }
+        if (lane == 0) {
+          p.lse_all[bh] = lse;
+          if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
+        }
+      } else {
+        // record 1 for the unit that begins in this run, record 0 for the one that began before it
+        float* rec = p.records + ((int64_t)w * 2 + (at.t + 1 == seg ? 1 : 0)) * REC;
+        if (lane == 0) *reinterpret_cast<float2*>(rec) = make_float2(m_ref, lsum);
+        if (quad == 0) {
+          reinterpret_cast<float4*>(rec + 4)[2 * part] = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
+          reinterpret_cast<float4*>(rec + 4)[2 * part + 1] = make_float4(acc[2].x, acc[2].y, acc[3].x, acc[3].y);
+        }
+      }
+      seg = 0;
+    }
+    if (i + 1 < count) at.next(p);
   }
-#pragma unroll
-  for (int d = 0; d < 8; ++d) {
-    acc[d] += __shfl_xor_sync(0xffffffffu, acc[d], 8);
-    acc[d] += __shfl_xor_sync(0xffffffffu, acc[d], 16);
-  }
-  lsum += __shfl_xor_sync(0xffffffffu, lsum, 8);
-  lsum += __shfl_xor_sync(0xffffffffu, lsum, 16);
-  if (sub == 0) {
-#pragma unroll
-    for (int d = 0; d < 8; ++d) s_acc[warp][8 * part + d] = acc[d];
-  }
-  if (lane == 0) { s_m[warp] = m_ref; s_l[warp] = lsum; }
-  __syncthreads();
-  float m = s_m[0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w]);
-  float* out = p.ws + ((int64_t)split * p.B * p.H + bh) * 66;
-  if (tid < 64) {
-    float a = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) a = fmaf(s_acc[w][tid], (s_m[w] == -INFINITY) ? (s_l[w] != s_l[w] ? s_l[w] : 0.f) : exp2f(s_m[w] - m), a);
-    out[2 + tid] = a;
-  }
-  if (tid == 0) {
-    float l = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) l = fmaf(s_l[w], (s_m[w] == -INFINITY) ? (s_l[w] != s_l[w] ? s_l[w] : 0.f) : exp2f(s_m[w] - m), l);
-    out[0] = m;
-    out[1] = l;
+  if (!ok) {                                    // a wait ran out: let the copies in flight land before leaving
+    for (int s = 0; s < NSTAGE && s < filled; ++s)
+      mbar_wait<true>(bars + 8 * s, (uint32_t)((filled - 1 - s) / NSTAGE) & 1, p.status);
   }
 }
 
-// One block per (batch, head): merge the splits in order, write y and lse, then add the weights.
+// The records of one unit, merged by a warp in worker order: m and lse, and with kOut lanes hold head
+// dims 2 lane, 2 lane + 1 of the output. Returns false for a unit that one worker finished (or that has
+// no keys); n is its number of keys.
+template <bool kOut>
+__device__ __forceinline__ bool join_unit(const PagedAttnParams& p, int b, int h, int64_t n, float& lse, float2& out) {
+  const int lane = threadIdx.x & 31;
+  int64_t all;
+  const int64_t T = (n + TK - 1) / TK, u0 = tiles_before(p, b, all) * p.H + h * T, tiles = all * p.H;
+  if (T == 0) return false;
+  const int w0 = worker_of(u0, tiles), w1 = worker_of(u0 + T - 1, tiles);
+  if (w0 == w1) return false;
+  auto rec = [&](int w) { return p.records + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * REC; };
+  float m = -INFINITY;
+  for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, rec(w)[0]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float mb = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float2 a = bcast2(0.f);
+  for (int c0 = w0; c0 <= w1; c0 += 32) {
+    float sc = 0.f;
+    if (c0 + lane <= w1) {
+      const float2 ml = *reinterpret_cast<const float2*>(rec(c0 + lane));
+      sc = exp2f(ml.x - mb);
+      l = fmaf(ml.y, sc, l);
+    }
+    if constexpr (kOut) {
+      const int cnt = min(32, w1 - c0 + 1);
+#pragma unroll 4
+      for (int i = 0; i < cnt; ++i)
+        a = fma2(*reinterpret_cast<const float2*>(rec(c0 + i) + 4 + 2 * lane), bcast2(__shfl_sync(0xffffffffu, sc, i)), a);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  lse = m + log2f(l);
+  out = mul2(a, bcast2(1.f / l));
+  return true;
+}
+
+// One warp per unit: y and lse of the units that several workers share, and of the rows with no keys.
 template <bool kHalf>
-__global__ void __launch_bounds__(NT) paged_join_kernel(PagedAttnParams p) {
-  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, tid = threadIdx.x;
-  const int64_t N = keys_of(p, b), stride = (int64_t)p.B * p.H * 66;
-  const float* rec = p.ws + (int64_t)bh * 66;
-  float m = -INFINITY, l = 0.f, a = 0.f;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, rec[s * stride]);
-  for (int s = 0; s < p.splits; ++s) {
-    const float ms = rec[s * stride], ls = rec[s * stride + 1];
-    const float sc = (ms == -INFINITY) ? (ls != ls ? ls : 0.f) : exp2f(ms - m);
-    l = fmaf(ls, sc, l);
-    if (tid < 64) a = fmaf(rec[s * stride + 2 + tid], sc, a);
+__device__ __forceinline__ void finish_unit(const PagedAttnParams& p, int64_t bh) {
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H), lane = threadIdx.x & 31;
+  const int64_t n = keys_of(p, b);
+  float lse = -INFINITY;
+  float2 out = bcast2(0.f);
+  if (!join_unit<true>(p, b, h, n, lse, out) && n > 0) return;
+  reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = pack2<kHalf>(out.x, out.y);
+  if (lane == 0) {
+    p.lse_all[bh] = lse;
+    if (n > 0 && !isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
   }
-  const float lse = (N == 0) ? -INFINITY : m + log2f(l);
-  if (tid < 64) {
-    const float y = (N == 0) ? 0.f : a / l;
-    const uint32_t w = pack2<kHalf>(y, 0.f);
-    reinterpret_cast<uint16_t*>(p.y + 2 * ((int64_t)b * p.y_sb + (int64_t)h * p.y_sh))[tid] = (uint16_t)w;
-  }
-  if (tid == 0) {
-    if (p.lse) p.lse[bh] = lse;
-    if (N > 0 && !isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
-  }
-  if (!p.weight_out) return;
-  const float* xs = p.ws + (int64_t)p.splits * stride + (int64_t)bh * p.max_keys;
-  for (int64_t j = tid; j < N; j += NT) {
+}
+
+template <bool kHalf>
+__global__ void __launch_bounds__(128) paged_join_kernel(PagedAttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t bh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (bh < (int64_t)p.B * p.H) finish_unit<kHalf>(p, bh);
+}
+
+// weight_out_j = weight_j + 2^(x_j - lse), four keys per thread (a page holds a multiple of four), one unit
+// and 1024 keys per block; the first block of a unit also finishes it.
+constexpr int WT = 256;
+template <bool kHalf>
+__global__ void __launch_bounds__(WT) paged_weights_kernel(PagedAttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t bh = blockIdx.y;
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
+  if (blockIdx.x == 0 && threadIdx.x < 32) finish_unit<kHalf>(p, bh);
+  const int64_t n = keys_of(p, b);
+  for (int64_t j0 = (int64_t)blockIdx.x * WT * 4; j0 < n; j0 += (int64_t)gridDim.x * WT * 4) {
+    float lse;
+    float2 unused;
+    if (!join_unit<false>(p, b, h, n, lse, unused)) lse = p.lse_all[bh];
+    const int64_t j = j0 + threadIdx.x * 4;
+    if (j >= n) continue;
     const int page = page_of(p.pg, b, j, nullptr);
     if (page < 0) continue;
     const int64_t at = page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
-    p.weight_out[at] = p.pg.weight[at] + exp2f(xs[j] - lse);
+    const float* xs = p.scores + bh * p.max_keys + j;
+    if (j + 4 <= n) {
+      const float4 x = *reinterpret_cast<const float4*>(xs);
+      float4 wv = *reinterpret_cast<const float4*>(p.pg.weight + at);
+      wv.x += exp2f(x.x - lse); wv.y += exp2f(x.y - lse); wv.z += exp2f(x.z - lse); wv.w += exp2f(x.w - lse);
+      *reinterpret_cast<float4*>(p.weight_out + at) = wv;
+    } else {
+      for (int e = 0; j + e < n; ++e) p.weight_out[at + e] = p.pg.weight[at + e] + exp2f(xs[e] - lse);
+    }
   }
+}
+
+// A kernel launched so that its blocks may be resident before the previous kernel of the stream ends
+// (they wait for it themselves).
+template <typename K>
+cudaError_t launch_after(K kernel, dim3 grid, int threads, cudaStream_t st, const PagedAttnParams& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <bool kHalf>
+cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
+  auto* main = p.weight_out ? paged_attn_kernel<kHalf, true> : paged_attn_kernel<kHalf, false>;
+  cudaError_t e = cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+  if (e != cudaSuccess) return e;
+  main<<<NCTA, NW * 32, SMEM_BYTES, st>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  const int units = p.B * p.H;
+  if (!p.weight_out) return launch_after(paged_join_kernel<kHalf>, dim3((units + 3) / 4), 128, st, p);
+  const int64_t chunks = (p.max_keys + WT * 4 - 1) / (WT * 4);
+  return launch_after(paged_weights_kernel<kHalf>, dim3((unsigned)(chunks < 65535 ? chunks : 65535), units), WT, st, p);
 }
 
 }  // namespace pat
 
-int paged_attn_splits(int64_t B, int64_t H, int64_t max_keys) {
-  int64_t s = (148 * 8 * 4 + B * H - 1) / (B * H);
-  const int64_t most = (max_keys + pat::NT - 1) / pat::NT;
-  if (s > most) s = most;
-  return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+int64_t paged_attn_workspace_floats(int64_t units, int64_t max_keys, bool scores) {
+  const int64_t base = (int64_t)pat::NWORK * 2 * pat::REC + ((units + 3) & ~int64_t(3));
+  return base + (scores ? units * max_keys : 0);
 }
 
-cudaError_t launch_paged_attn(const PagedAttnParams& p, int dtype, cudaStream_t st) {
-  dim3 grid(p.splits, p.B * p.H);
-  if (dtype == 1) {
-    pat::paged_split_kernel<true><<<grid, pat::NT, 0, st>>>(p);
-    pat::paged_join_kernel<true><<<p.B * p.H, pat::NT, 0, st>>>(p);
-  } else {
-    pat::paged_split_kernel<false><<<grid, pat::NT, 0, st>>>(p);
-    pat::paged_join_kernel<false><<<p.B * p.H, pat::NT, 0, st>>>(p);
-  }
-  return cudaGetLastError();
+cudaError_t launch_paged_attn(PagedAttnParams p, int dtype, cudaStream_t st) {
+  const int64_t units = (int64_t)p.B * p.H;
+  p.records = p.ws;
+  p.lse_all = p.lse ? p.lse : p.ws + (int64_t)pat::NWORK * 2 * pat::REC;
+  p.scores = p.ws + paged_attn_workspace_floats(units, 0, false);
+  return dtype == 1 ? pat::launch<true>(p, st) : pat::launch<false>(p, st);
 }
 
 }  // namespace sisa

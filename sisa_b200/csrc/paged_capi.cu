@@ -67,8 +67,7 @@ int launched(cudaError_t e, const char* what) {
 extern "C" {
 
 int64_t sisa_paged_attn_workspace(int64_t B, int64_t H, int64_t max_keys, int accumulate) {
-  const int64_t rec = (int64_t)sisa::paged_attn_splits(B, H, max_keys) * B * H * 66;
-  return 4 * (rec + (accumulate ? B * H * max_keys : 0));
+  return 4 * sisa::paged_attn_workspace_floats(B * H, max_keys, accumulate != 0);
 }
 
 int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, const float* f_q,
@@ -94,7 +93,6 @@ int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, 
   p.y = static_cast<char*>(y->data); p.y_sb = y->stride_b; p.y_sh = y->stride_h;
   p.lse = lse; p.weight_out = weight_out; p.ws = static_cast<float*>(workspace);
   p.B = (int)B; p.H = (int)H; p.max_keys = max_pages * pages->page_size;
-  p.splits = sisa::paged_attn_splits(B, H, p.max_keys);
   p.status = status;
   return launched(sisa::launch_paged_attn(p, dtype, static_cast<cudaStream_t>(stream)), what);
 }
