@@ -14,9 +14,10 @@
 // (16 bytes of its rows each), so a tile is eight groups of four keys; the eight partial dot products of a
 // lane are summed by a reduce-scatter over the eight lanes, after which every lane owns one key's score and
 // the exponentials are taken once per key.
-// A unit inside one warp's run is finished there; the others leave (m, l, acc) records, at most two per
-// warp, that paged_join_kernel merges in warp order (deterministic, no atomics). With weights, the scores
-// are kept in the workspace (4 bytes per key) and paged_weights_kernel adds the shares once lse is known.
+// A unit inside one warp's run is finished there. The pieces of the others are merged at the end of the CTA,
+// whose warps' runs are neighbours; what reaches past the CTA leaves as (m, l, acc) records, at most two per
+// CTA, that paged_join_kernel merges in order (deterministic, no atomics). With weights, the scores are kept
+// in the workspace (4 bytes per key) and paged_weights_kernel adds the shares once lse is known.
 #include <cuda_runtime.h>
 #include <cstdint>
 
@@ -27,15 +28,17 @@ namespace sisa {
 namespace pat {
 
 constexpr int TK = 32;                          // keys per tile
-constexpr int NW = 4, NSTAGE = 5;               // warps per CTA, ring stages per warp
-constexpr int NCTA = 148, NWORK = NCTA * NW;    // one CTA per SM
+constexpr int NW = 5, NSTAGE = 2;               // warps per CTA, ring stages per warp; two CTAs per SM
+constexpr int NCTA = 148 * 16;                  // eight waves: SMs stream at different rates, and the ones
+                                                // that are done take the next CTA
+constexpr int NWORK = NCTA * NW, WMIN = 296 * NW, GRAIN = 16;
 constexpr uint32_t OFF_V = TK * 128, OFF_B = OFF_V + TK * 128, OFF_G = OFF_B + TK * 64, OFF_F = OFF_G + TK * 4;
+constexpr int REC = 68;                         // floats of a record: m, l, 2 unused, acc[64]
 constexpr uint32_t SZ_STAGE = OFF_F + TK * 4;   // 10,496 bytes
 constexpr uint32_t SZ_WARP = NSTAGE * SZ_STAGE;
-constexpr uint32_t OFF_BAR = NW * SZ_WARP, OFF_MASK = OFF_BAR + NW * NSTAGE * 8;
+constexpr uint32_t OFF_REC = NW * SZ_WARP, OFF_BAR = OFF_REC + NW * 2 * REC * 4, OFF_MASK = OFF_BAR + NW * NSTAGE * 8;
 constexpr uint32_t SMEM_BYTES = OFF_MASK + NW * NSTAGE * 4 + 128;
-static_assert(SZ_STAGE % 128 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory");
-constexpr int REC = 68;                         // floats of a record: m, l, 2 unused, acc[64]
+static_assert(SZ_STAGE % 128 == 0 && 2 * (SMEM_BYTES + 1024) <= 228 * 1024, "shared memory");
 
 __device__ __forceinline__ int64_t keys_of(const PagedAttnParams& p, int b) {
   const int64_t n = __ldg(p.lengths + b);
@@ -60,9 +63,14 @@ __device__ __forceinline__ int64_t tiles_before(const PagedAttnParams& p, int b,
   return before;
 }
 
-// The line is shared by min(NWORK, tiles) workers, so none of them has an empty run: worker w takes the tiles
-// [run_start(w), run_start(w + 1)); worker_of is its inverse.
-__device__ __forceinline__ int64_t workers(int64_t tiles) { return tiles < NWORK ? tiles : NWORK; }
+// The line is shared by one worker (warp) per tile while there are few tiles, then by the warps of one wave,
+// and beyond GRAIN tiles a worker by more whole waves, up to eight; none has an empty run. Worker w takes the
+// tiles [run_start(w), run_start(w + 1)); worker_of is its inverse.
+__device__ __forceinline__ int64_t workers(int64_t tiles) {
+  if (tiles < WMIN) return tiles;
+  const int64_t waves = tiles / (WMIN * GRAIN);
+  return waves < 1 ? WMIN : (waves < 8 ? waves * WMIN : NWORK);
+}
 __device__ __forceinline__ int64_t run_start(int64_t w, int64_t tiles) { return w * tiles / workers(tiles); }
 __device__ __forceinline__ int worker_of(int64_t x, int64_t tiles) {
   return (int)(((x + 1) * workers(tiles) - 1) / tiles);
@@ -131,8 +139,38 @@ __device__ __forceinline__ float reduce_scatter8(const float (&v)[8], int part) 
   return (hi ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, hi ? c[0] : c[1], 1);
 }
 
+// A softmax sum held by a warp: maximum, sum, and head dims 2 lane, 2 lane + 1 of the weighted values.
+struct Sum {
+  float m, l;
+  float2 a;
+  __device__ __forceinline__ void clear() { m = -INFINITY; l = 0.f; a = make_float2(0.f, 0.f); }
+  __device__ __forceinline__ void add(float2 ml, float2 v) {
+    const float mn = fmaxf(m, ml.x), mb = mn == -INFINITY ? 0.f : mn;
+    const float s0 = exp2f(m - mb), s1 = exp2f(ml.x - mb);
+    l = fmaf(ml.y, s1, l * s0);
+    a = fma2(v, bcast2(s1), mul2(a, bcast2(s0)));
+    m = mn;
+  }
+  __device__ __forceinline__ void add(const float* rec) {
+    add(*reinterpret_cast<const float2*>(rec), *reinterpret_cast<const float2*>(rec + 4 + 2 * (threadIdx.x & 31)));
+  }
+};
+
+// y and lse of unit bh = (b, h) from its complete sum.
+template <bool kHalf>
+__device__ __forceinline__ void write_row(const PagedAttnParams& p, int64_t bh, const Sum& s) {
+  const int64_t b = bh / p.H, h = bh % p.H;
+  const int lane = threadIdx.x & 31;
+  const float lse = s.m + log2f(s.l), r = 1.f / s.l;
+  reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = pack2<kHalf>(s.a.x * r, s.a.y * r);
+  if (lane == 0) {
+    p.lse_all[bh] = lse;
+    if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
+  }
+}
+
 template <bool kHalf, bool kScores>
-__global__ void __launch_bounds__(NW * 32, 1) paged_attn_kernel(PagedAttnParams p) {
+__global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -149,14 +187,21 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_attn_kernel(PagedAttnParams 
 
   int64_t per_head;
   tiles_before(p, 0, per_head);
-  const int64_t tiles = per_head * p.H;
-  const int w = blockIdx.x + NCTA * warp;       // a short line is spread over the SMs first
+  const int64_t tiles = per_head * p.H, nwork = workers(tiles);
+  if ((int64_t)blockIdx.x * NW >= nwork && blockIdx.x > 0) return;
+  const int w = blockIdx.x * NW + warp;
   if (w == 0) {                                 // lengths past the table, once per sequence
     for (int b = lane; b < p.B; b += 32)
       if (__ldg(p.lengths + b) > p.max_keys && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
   }
-  if (w >= workers(tiles)) return;
-  const int64_t x0 = run_start(w, tiles), count = run_start(w + 1, tiles) - x0;
+  // the pieces this warp leaves for the CTA's merge: [0] of the unit that began before its run (s_ends: and
+  // ends in it), [1] of the one that goes on after it; s_unit -1: none
+  __shared__ int64_t s_unit[NW][2];
+  __shared__ bool s_ends[NW];
+  float* pieces = reinterpret_cast<float*>(gbase + OFF_REC);
+  if (lane == 0) { s_unit[warp][0] = s_unit[warp][1] = -1; s_ends[warp] = false; }
+  __syncwarp();
+  const int64_t x0 = w < nwork ? run_start(w, tiles) : 0, count = w < nwork ? run_start(w + 1, tiles) - x0 : 0;
 
   // ---- this lane's part of a tile's copies: operand op of the tile's sub-tile sub (pages of 16 slots
   // give a tile two sub-tiles)
@@ -175,13 +220,15 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_attn_kernel(PagedAttnParams 
   const bool copier = sub < nsub && row_bytes > 0;
   const uint32_t key_bytes = 128 + 128 + 64 + 4 + (p.f_q ? 4 : 0);
 
-  Cursor in = find_tile(p, x0), at = in;
+  Cursor in{}, at;
+  if (count > 0) in = find_tile(p, x0);
+  at = in;
   // the page of this lane's sub-tile at the fill cursor, read one tile ahead of its use
   auto page_at = [&]() {
     const int64_t j = in.t * TK + sub * rows_max;
     return sub < nsub && j < in.n ? __ldg(p.pg.table + (int64_t)in.b * p.pg.table_sb + (j >> p.pg.page_shift)) : -1;
   };
-  int page = page_at();
+  int page = count > 0 ? page_at() : -1;
   int64_t filled = 0;
   auto fill = [&](int s) {
     const int64_t j = in.t * TK + sub * rows_max;
@@ -320,9 +367,13 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_attn_kernel(PagedAttnParams 
           if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
         }
       } else {
-        // record 1 for the unit that begins in this run, record 0 for the one that began before it
-        float* rec = p.records + ((int64_t)w * 2 + (at.t + 1 == seg ? 1 : 0)) * REC;
-        if (lane == 0) *reinterpret_cast<float2*>(rec) = make_float2(m_ref, lsum);
+        const int kind = at.t + 1 == seg ? 1 : 0;
+        float* rec = pieces + (warp * 2 + kind) * REC;
+        if (lane == 0) {
+          *reinterpret_cast<float2*>(rec) = make_float2(m_ref, lsum);
+          s_unit[warp][kind] = bh;
+          if (kind == 0) s_ends[warp] = at.t + 1 == at.T;
+        }
         if (quad == 0) {
           reinterpret_cast<float4*>(rec + 4)[2 * part] = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
           reinterpret_cast<float4*>(rec + 4)[2 * part + 1] = make_float4(acc[2].x, acc[2].y, acc[3].x, acc[3].y);
@@ -336,84 +387,123 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_attn_kernel(PagedAttnParams 
     for (int s = 0; s < NSTAGE && s < filled; ++s)
       mbar_wait<true>(bars + 8 * s, (uint32_t)((filled - 1 - s) / NSTAGE) & 1, p.status);
   }
+  // ---- the CTA's runs are neighbours: one warp merges their pieces in order. What began before the CTA or
+  // goes on after it becomes its record 0 or 1.
+  __syncthreads();
+  if (warp != 0) return;
+  Sum sum;
+  int64_t unit = -1;                            // the unit being merged, -1: none
+  bool before = false;                          // it began before this CTA
+  auto close = [&](bool ends) {
+    if (ends && !before) {
+      write_row<kHalf>(p, unit, sum);
+    } else {
+      float* rec = p.records + ((int64_t)blockIdx.x * 2 + (before ? 0 : 1)) * REC;
+      if (lane == 0) *reinterpret_cast<float2*>(rec) = make_float2(sum.m, sum.l);
+      *reinterpret_cast<float2*>(rec + 4 + 2 * lane) = sum.a;
+    }
+    unit = -1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < NW; ++i) {
+    if (s_unit[i][0] >= 0) {
+      if (unit < 0) { unit = s_unit[i][0]; before = true; sum.clear(); }
+      sum.add(pieces + (i * 2) * REC);
+      if (s_ends[i]) close(true);
+    }
+    if (s_unit[i][1] >= 0) {
+      unit = s_unit[i][1];
+      before = false;
+      sum.clear();
+      sum.add(pieces + (i * 2 + 1) * REC);
+    }
+  }
+  if (unit >= 0) close(false);
 }
 
-// The records of one unit, merged by a warp in worker order: m and lse, and with kOut lanes hold head
-// dims 2 lane, 2 lane + 1 of the output. Returns false for a unit that one worker finished (or that has
-// no keys); n is its number of keys.
-template <bool kOut>
-__device__ __forceinline__ bool join_unit(const PagedAttnParams& p, int b, int h, int64_t n, float& lse, float2& out) {
-  const int lane = threadIdx.x & 31;
+// The records of one unit, merged by the JW warps of a block: each takes a run of them (the maximum first,
+// then every record on its own, so that the loads are in flight together), and warp 0 the runs' sums, all in
+// CTA order. Returns false (to every warp) for a unit that one CTA finished or that has no keys; the sum is
+// warp 0's.
+constexpr int JW = 8;
+__device__ __forceinline__ bool join_unit(const PagedAttnParams& p, int b, int h, int64_t n, Sum& sum) {
   int64_t all;
   const int64_t T = (n + TK - 1) / TK, u0 = tiles_before(p, b, all) * p.H + h * T, tiles = all * p.H;
   if (T == 0) return false;
-  const int w0 = worker_of(u0, tiles), w1 = worker_of(u0 + T - 1, tiles);
-  if (w0 == w1) return false;
-  auto rec = [&](int w) { return p.records + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * REC; };
-  float m = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, rec(w)[0]);
+  const int c0 = worker_of(u0, tiles) / NW, c1 = worker_of(u0 + T - 1, tiles) / NW;
+  if (c0 == c1) return false;
+  __shared__ __align__(16) float s_sum[JW][REC];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (c1 - c0 + JW) / JW, lo = c0 + warp * per, hi = min(c1 + 1, lo + per);
+  auto rec = [&](int c) { return p.records + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * REC; };
+  sum.clear();
+  for (int c = lo; c < hi; c += 32) {
+    const float2 ml = c + lane < hi ? *reinterpret_cast<const float2*>(rec(c + lane)) : make_float2(-INFINITY, 0.f);
+    float m = ml.x;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float mb = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float2 a = bcast2(0.f);
-  for (int c0 = w0; c0 <= w1; c0 += 32) {
-    float sc = 0.f;
-    if (c0 + lane <= w1) {
-      const float2 ml = *reinterpret_cast<const float2*>(rec(c0 + lane));
-      sc = exp2f(ml.x - mb);
-      l = fmaf(ml.y, sc, l);
-    }
-    if constexpr (kOut) {
-      const int cnt = min(32, w1 - c0 + 1);
-#pragma unroll 4
-      for (int i = 0; i < cnt; ++i)
-        a = fma2(*reinterpret_cast<const float2*>(rec(c0 + i) + 4 + 2 * lane), bcast2(__shfl_sync(0xffffffffu, sc, i)), a);
-    }
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float sc = exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+    float l = ml.y * sc;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float2 a = bcast2(0.f);
+    const int cnt = min(32, hi - c);
+#pragma unroll 8
+    for (int i = 0; i < cnt; ++i)
+      a = fma2(*reinterpret_cast<const float2*>(rec(c + i) + 4 + 2 * lane), bcast2(__shfl_sync(0xffffffffu, sc, i)), a);
+    sum.add(make_float2(m, l), a);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  lse = m + log2f(l);
-  out = mul2(a, bcast2(1.f / l));
+  if (lane == 0) *reinterpret_cast<float2*>(s_sum[warp]) = make_float2(sum.m, sum.l);
+  *reinterpret_cast<float2*>(s_sum[warp] + 4 + 2 * lane) = sum.a;
+  __syncthreads();
+  if (warp == 0)
+    for (int i = 1; i < JW; ++i) sum.add(s_sum[i]);
   return true;
 }
 
-// One warp per unit: y and lse of the units that several workers share, and of the rows with no keys.
+// y and lse of a unit that several CTAs share, or of a row with no keys, by one warp.
 template <bool kHalf>
-__device__ __forceinline__ void finish_unit(const PagedAttnParams& p, int64_t bh) {
-  const int b = (int)(bh / p.H), h = (int)(bh % p.H), lane = threadIdx.x & 31;
-  const int64_t n = keys_of(p, b);
-  float lse = -INFINITY;
-  float2 out = bcast2(0.f);
-  if (!join_unit<true>(p, b, h, n, lse, out) && n > 0) return;
-  reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = pack2<kHalf>(out.x, out.y);
-  if (lane == 0) {
-    p.lse_all[bh] = lse;
-    if (n > 0 && !isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
+__device__ __forceinline__ void finish_unit(const PagedAttnParams& p, int64_t bh, int64_t n, bool joined, const Sum& sum) {
+  const int64_t b = bh / p.H, h = bh % p.H;
+  const int lane = threadIdx.x & 31;
+  if (joined) {
+    write_row<kHalf>(p, bh, sum);
+  } else if (n == 0) {
+    reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = 0u;
+    if (lane == 0) p.lse_all[bh] = -INFINITY;
   }
 }
 
 template <bool kHalf>
-__global__ void __launch_bounds__(128) paged_join_kernel(PagedAttnParams p) {
+__global__ void __launch_bounds__(JW * 32) paged_join_kernel(PagedAttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t bh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (bh < (int64_t)p.B * p.H) finish_unit<kHalf>(p, bh);
+  const int64_t bh = blockIdx.x;
+  const int64_t n = keys_of(p, (int)(bh / p.H));
+  Sum sum;
+  const bool joined = join_unit(p, (int)(bh / p.H), (int)(bh % p.H), n, sum);
+  if (threadIdx.x < 32) finish_unit<kHalf>(p, bh, n, joined, sum);
 }
 
 // weight_out_j = weight_j + 2^(x_j - lse), four keys per thread (a page holds a multiple of four), one unit
 // and 1024 keys per block; the first block of a unit also finishes it.
-constexpr int WT = 256;
+constexpr int WT = JW * 32;
 template <bool kHalf>
 __global__ void __launch_bounds__(WT) paged_weights_kernel(PagedAttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t bh = blockIdx.y;
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
-  if (blockIdx.x == 0 && threadIdx.x < 32) finish_unit<kHalf>(p, bh);
   const int64_t n = keys_of(p, b);
+  if (blockIdx.x > 0 && (int64_t)blockIdx.x * WT * 4 >= n) return;
+  __shared__ float s_lse;
+  Sum sum;
+  const bool joined = join_unit(p, b, h, n, sum);
+  if (threadIdx.x < 32) {
+    if (blockIdx.x == 0) finish_unit<kHalf>(p, bh, n, joined, sum);
+    if (threadIdx.x == 0 && n > 0) s_lse = joined ? sum.m + log2f(sum.l) : p.lse_all[bh];
+  }
+  __syncthreads();
+  const float lse = s_lse;
   for (int64_t j0 = (int64_t)blockIdx.x * WT * 4; j0 < n; j0 += (int64_t)gridDim.x * WT * 4) {
-    float lse;
-    float2 unused;
-    if (!join_unit<false>(p, b, h, n, lse, unused)) lse = p.lse_all[bh];
     const int64_t j = j0 + threadIdx.x * 4;
     if (j >= n) continue;
     const int page = page_of(p.pg, b, j, nullptr);
@@ -455,7 +545,7 @@ cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
   main<<<NCTA, NW * 32, SMEM_BYTES, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int units = p.B * p.H;
-  if (!p.weight_out) return launch_after(paged_join_kernel<kHalf>, dim3((units + 3) / 4), 128, st, p);
+  if (!p.weight_out) return launch_after(paged_join_kernel<kHalf>, dim3(units), JW * 32, st, p);
   const int64_t chunks = (p.max_keys + WT * 4 - 1) / (WT * 4);
   return launch_after(paged_weights_kernel<kHalf>, dim3((unsigned)(chunks < 65535 ? chunks : 65535), units), WT, st, p);
 }
@@ -463,14 +553,14 @@ cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
 }  // namespace pat
 
 int64_t paged_attn_workspace_floats(int64_t units, int64_t max_keys, bool scores) {
-  const int64_t base = (int64_t)pat::NWORK * 2 * pat::REC + ((units + 3) & ~int64_t(3));
+  const int64_t base = (int64_t)pat::NCTA * 2 * pat::REC + ((units + 3) & ~int64_t(3));
   return base + (scores ? units * max_keys : 0);
 }
 
 cudaError_t launch_paged_attn(PagedAttnParams p, int dtype, cudaStream_t st) {
   const int64_t units = (int64_t)p.B * p.H;
   p.records = p.ws;
-  p.lse_all = p.lse ? p.lse : p.ws + (int64_t)pat::NWORK * 2 * pat::REC;
+  p.lse_all = p.lse ? p.lse : p.ws + (int64_t)pat::NCTA * 2 * pat::REC;
   p.scores = p.ws + paged_attn_workspace_floats(units, 0, false);
   return dtype == 1 ? pat::launch<true>(p, st) : pat::launch<false>(p, st);
 }
