@@ -119,6 +119,19 @@ __device__ __forceinline__ Cursor find_tile(const PagedAttnParams& p, int64_t x)
   }
 }
 
+// A bulk copy whose lines L2 may drop first: the keys are read once, and what should stay in L2 is the
+// scores that the weights pass reads back.
+__device__ __forceinline__ uint64_t policy_evict_first() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
+}
+__device__ __forceinline__ void bulk_load_hint(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t pol) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+      ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(pol) : "memory");
+}
+
 template <bool kHalf>
 __device__ __forceinline__ float2 unpack2(uint32_t w) { return make_float2(unpack_lo<kHalf>(w), unpack_hi<kHalf>(w)); }
 
@@ -230,6 +243,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
   };
   int page = count > 0 ? page_at() : -1;
   int64_t filled = 0;
+  const uint64_t policy = policy_evict_first();
   auto fill = [&](int s) {
     const int64_t j = in.t * TK + sub * rows_max;
     const int left = (int)(in.n - j < rows_max ? in.n - j : rows_max);       // keys of this sub-tile
@@ -246,9 +260,9 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
     }
     __syncwarp();
     if (copier && rows > 0)
-      bulk_load(ring + s * SZ_STAGE + dst_off,
+      bulk_load_hint(ring + s * SZ_STAGE + dst_off,
                 src0 + page * src_p + in.h * src_h + (j & ((1 << p.pg.page_shift) - 1)) * row_bytes,
-                (uint32_t)(rows * row_bytes), bars + 8 * s);
+                (uint32_t)(rows * row_bytes), bars + 8 * s, policy);
     ++filled;
     if (filled < count) {
       in.next(p);
@@ -484,16 +498,30 @@ __global__ void __launch_bounds__(JW * 32) paged_join_kernel(PagedAttnParams p) 
   if (threadIdx.x < 32) finish_unit<kHalf>(p, bh, n, joined, sum);
 }
 
-// weight_out_j = weight_j + 2^(x_j - lse), four keys per thread (a page holds a multiple of four), one unit
-// and 1024 keys per block; the first block of a unit also finishes it.
+// weight_out_j = weight_j + 2^(x_j - lse), four keys per thread and step (a page holds a multiple of four).
+// A unit has gridDim.x blocks, each with every gridDim.x-th run of 1024 keys; the first one also finishes the
+// unit. The loads of a block's first step do not need lse and are issued ahead of the join.
 constexpr int WT = JW * 32;
 template <bool kHalf>
 __global__ void __launch_bounds__(WT) paged_weights_kernel(PagedAttnParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t bh = blockIdx.y;
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
-  const int64_t n = keys_of(p, b);
+  const int64_t n = keys_of(p, b), step = (int64_t)gridDim.x * WT * 4;
   if (blockIdx.x > 0 && (int64_t)blockIdx.x * WT * 4 >= n) return;
+  const float* xs = p.scores + bh * p.max_keys;
+  struct Four { int64_t at; float4 x, w; };      // at < 0: nothing to do
+  auto place = [&](int64_t j) -> int64_t {
+    if (j >= n) return -1;
+    const int page = page_of(p.pg, b, j, nullptr);
+    return page < 0 ? -1 : page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
+  };
+  int64_t j = (int64_t)blockIdx.x * WT * 4 + threadIdx.x * 4;
+  // the last four of a unit may reach past its end: those slots are the page's own and are not stored
+  Four f;
+  f.at = place(j);
+  f.w = f.at >= 0 ? *reinterpret_cast<const float4*>(p.pg.weight + f.at) : make_float4(0.f, 0.f, 0.f, 0.f);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  f.x = f.at >= 0 ? *reinterpret_cast<const float4*>(xs + j) : make_float4(0.f, 0.f, 0.f, 0.f);
   __shared__ float s_lse;
   Sum sum;
   const bool joined = join_unit(p, b, h, n, sum);
@@ -503,21 +531,26 @@ __global__ void __launch_bounds__(WT) paged_weights_kernel(PagedAttnParams p) {
   }
   __syncthreads();
   const float lse = s_lse;
-  for (int64_t j0 = (int64_t)blockIdx.x * WT * 4; j0 < n; j0 += (int64_t)gridDim.x * WT * 4) {
-    const int64_t j = j0 + threadIdx.x * 4;
-    if (j >= n) continue;
-    const int page = page_of(p.pg, b, j, nullptr);
-    if (page < 0) continue;
-    const int64_t at = page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
-    const float* xs = p.scores + bh * p.max_keys + j;
-    if (j + 4 <= n) {
-      const float4 x = *reinterpret_cast<const float4*>(xs);
-      float4 wv = *reinterpret_cast<const float4*>(p.pg.weight + at);
-      wv.x += exp2f(x.x - lse); wv.y += exp2f(x.y - lse); wv.z += exp2f(x.z - lse); wv.w += exp2f(x.w - lse);
-      *reinterpret_cast<float4*>(p.weight_out + at) = wv;
-    } else {
-      for (int e = 0; j + e < n; ++e) p.weight_out[at + e] = p.pg.weight[at + e] + exp2f(xs[e] - lse);
+  for (; j - threadIdx.x * 4 < n; j += step) {
+    Four g;
+    g.at = place(j + step);
+    if (g.at >= 0) {
+      g.w = *reinterpret_cast<const float4*>(p.pg.weight + g.at);
+      g.x = *reinterpret_cast<const float4*>(xs + j + step);
     }
+    if (f.at >= 0) {
+      f.w.x += exp2f(f.x.x - lse); f.w.y += exp2f(f.x.y - lse);
+      f.w.z += exp2f(f.x.z - lse); f.w.w += exp2f(f.x.w - lse);
+      float* out = p.weight_out + f.at;
+      if (j + 4 <= n) {
+        *reinterpret_cast<float4*>(out) = f.w;
+      } else {
+        out[0] = f.w.x;
+        if (j + 1 < n) out[1] = f.w.y;
+        if (j + 2 < n) out[2] = f.w.z;
+      }
+    }
+    f = g;
   }
 }
 
@@ -546,8 +579,9 @@ cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int units = p.B * p.H;
   if (!p.weight_out) return launch_after(paged_join_kernel<kHalf>, dim3(units), JW * 32, st, p);
-  const int64_t chunks = (p.max_keys + WT * 4 - 1) / (WT * 4);
-  return launch_after(paged_weights_kernel<kHalf>, dim3((unsigned)(chunks < 65535 ? chunks : 65535), units), WT, st, p);
+  // about eight blocks per SM over all units, at most one per run of 1024 keys
+  const int64_t runs = (p.max_keys + WT * 4 - 1) / (WT * 4), want = (148 * 8 + units - 1) / units;
+  return launch_after(paged_weights_kernel<kHalf>, dim3((unsigned)(want < runs ? want : runs), units), WT, st, p);
 }
 
 }  // namespace pat
