@@ -6,6 +6,7 @@ The library is loaded on first use. If it has not been built, every CUDA entry p
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -87,8 +88,8 @@ class Pages(ctypes.Structure):
                 ("s_sp", _I64), ("s_sh", _I64), ("n_pages", _I64), ("page_size", _I64)]
 
 
-_PGP = ctypes.POINTER(Pages)
-
+# The views and pages of the paged-cache calls are declared as plain pointers: a call passes the struct's bytes
+# (view4_bytes), which costs a fraction of building a ctypes structure.
 # name -> (restype, argtypes); every symbol declared in include/sisa_b200.h
 SIGNATURES = {
     "sisa_version": (ctypes.c_char_p, []),
@@ -136,13 +137,13 @@ SIGNATURES = {
     "sisa_decode_attn_dpos": (_I, [_VP, _VP, _P, _P, _VP, _VP, _VP, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _I, _VP,
                                    _P, _P, _P]),
     "sisa_paged_attn_workspace": (_I64, [_I64, _I64, _I64, _I]),
-    "sisa_paged_attn": (_I, [_VP, _VP, _P, _P, _PGP, _P, _I64, _I64, _P, _P, _I64, _I64, _I, _VP, _P, _P, _P, _P, _P]),
-    "sisa_paged_evict": (_I, [_PGP, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
-    "sisa_paged_append": (_I, [_P, _I64, _P, _I64, _PGP, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _P,
+    "sisa_paged_attn": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I, _P, _P, _P, _P, _P, _P]),
+    "sisa_paged_evict": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "sisa_paged_append": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _P,
                                _P, _P, _P, _P]),
-    "sisa_attn_key_weights": (_I, [_VP, _VP, _VP, _VP, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "sisa_attn_key_weights": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P]),
     "sisa_paged_fill_workspace": (_I64, [_I64, _I64, _I64]),
-    "sisa_paged_fill": (_I, [_PGP, _P, _I64, _I64, _VP, _VP, _VP, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64,
+    "sisa_paged_fill": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64,
                              _I64, _I64, _P, _P, _P]),
     "sisa_rmsnorm_bwd_workspace": (_I64, [_I64, _I64]),
     "sisa_rmsnorm_fwd": (_I, [_P, _I64, _I, _P, _I64, _I64, ctypes.c_float, _P, _I64, _I, _P, _P, _P]),
@@ -226,11 +227,27 @@ def view4(t: torch.Tensor) -> View4:
     return View4(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
 
 
+_VIEW4 = struct.Struct("P3q")
+
+
+def view4_bytes(t: torch.Tensor) -> bytes:
+    """``sisa_view4`` of a 4-D tensor with a contiguous last axis (checked by the caller), as bytes."""
+    s = t.stride()
+    return _VIEW4.pack(t.data_ptr(), s[0], s[1], s[2])
+
+
 def vref(v: View4):
     return ctypes.byref(v)
 
 
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device | None = None) -> int:
+    """The raw handle of torch's current stream on ``device`` (without building a Stream object where torch
+    offers that: this runs once per call)."""
+    if _RAW_STREAM is not None and device is not None and device.index is not None:
+        return _RAW_STREAM(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -63,9 +63,11 @@ class KeyPages:
         self.k, self.v, self.b, self.g, self.f, self.weight, self.token = k, v, b, g, f, weight, token
         self.n_pages, self.n_head, self.page_size = P, H, S
         self.dtype, self.device = k.dtype, k.device
-        self._c = _lib.Pages(k.data_ptr(), v.data_ptr(), b.data_ptr(), g.data_ptr(), _lib.ptr(f), _lib.ptr(weight),
+        c = _lib.Pages(k.data_ptr(), v.data_ptr(), b.data_ptr(), g.data_ptr(), _lib.ptr(f), _lib.ptr(weight),
                              _lib.ptr(token), k.stride(0), k.stride(1), v.stride(0), v.stride(1), b.stride(0), b.stride(1),
                              g.stride(0), g.stride(1), P, S)
+        self.cbytes = bytes(c)                  # the struct every call passes
+        self.dev_index = k.device.index if k.device.index is not None else 0
 
     @classmethod
     def empty(cls, n_pages: int, n_head: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda",
@@ -80,47 +82,53 @@ class KeyPages:
         token = torch.empty(shape, dtype=torch.int32, device=device) if evict else None
         return cls(k, v, b, g, f, weight, token)
 
-    def cref(self):
-        return _lib.ctypes.byref(self._c)
-
 
 def _table(pages: KeyPages, table: Tensor, B: int) -> tuple[int, int, int]:
     """(pointer, row stride, max_pages) of a block table."""
-    if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or table.dtype != torch.int32:
-        raise ValueError(f"block_table must be ({B}, max_pages) int32, got {tuple(table.shape)} {table.dtype}")
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != B or shape[1] < 1 or table.dtype != torch.int32:
+        raise ValueError(f"block_table must be ({B}, max_pages) int32, got {tuple(shape)} {table.dtype}")
     if table.device != pages.device:
         raise ValueError(f"block_table is on {table.device}, the pages on {pages.device}")
-    if table.stride(1) != 1 and table.shape[1] > 1:
+    row, one = table.stride()
+    if one != 1 and shape[1] > 1:
         raise ValueError("block_table rows must be contiguous")
-    return table.data_ptr(), max(table.stride(0), table.shape[1]) if B == 1 else table.stride(0), table.shape[1]
+    return table.data_ptr(), (row if B > 1 else max(row, shape[1])), shape[1]
 
 
-def _rows(t: Tensor, shape: tuple, name: str, pages: KeyPages) -> Tensor:
-    """An int32 row tensor (positions, lengths, slots), checked."""
-    if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != pages.device:
+def _rows(t: Tensor, shape: tuple, name: str, pages: KeyPages) -> int:
+    """The pointer of an int32 row tensor (positions, lengths, slots), checked."""
+    if t.shape != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != pages.device:
         raise ValueError(f"{name} must be a contiguous {shape} int32 tensor on {pages.device}, got {tuple(t.shape)} "
                          f"{t.dtype} on {t.device}")
-    return t
+    return t.data_ptr()
 
 
 def _operand(t: Tensor) -> Tensor:
     """``t`` as the kernels read it: unit last stride, 16-byte aligned rows."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 0 for s in t.stride()[:-1]) \
-        and t.stride(-2) > 0
-    return t if ok else t.contiguous()
+    a, b, c, d = t.stride()
+    if d == 1 and (a | b | c) % 8 == 0 and c > 0 and a >= 0 and b >= 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.contiguous()
+
+
+def _f32(t: Tensor) -> Tensor:
+    """``t`` in fp32, contiguous."""
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _check_query(q: Tensor, c: Tensor, pages: KeyPages) -> tuple[int, int]:
-    if q.dim() != 4 or q.shape[2] != 1 or q.shape[3] != 64 or tuple(c.shape) != (q.shape[0], q.shape[1], 1, 32):
-        raise ValueError(f"paged_attention takes one query row with d_head 64 and d_state 32, got {tuple(q.shape)} and "
+    shape, H = q.shape, pages.n_head
+    if len(shape) != 4 or shape[2] != 1 or shape[3] != 64 or c.shape != (shape[0], shape[1], 1, 32):
+        raise ValueError(f"paged_attention takes one query row with d_head 64 and d_state 32, got {tuple(shape)} and "
                          f"{tuple(c.shape)}")
-    if q.shape[1] != pages.n_head:
-        raise ValueError(f"q has {q.shape[1]} heads, the pages {pages.n_head}")
+    if shape[1] != H:
+        raise ValueError(f"q has {shape[1]} heads, the pages {H}")
     if q.dtype != pages.dtype:
         raise TypeError(f"q dtype {q.dtype} differs from the pages' {pages.dtype}")
-    if q.device != pages.device:
-        raise ValueError(f"q is on {q.device}, the pages on {pages.device}")
-    return q.shape[0], q.shape[1]
+    if q.device != pages.device or c.device != pages.device:
+        raise ValueError(f"q and c are on {q.device} and {c.device}, the pages on {pages.device}")
+    return shape[0], H
 
 
 def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages: KeyPages, block_table: Tensor,
@@ -135,37 +143,38 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
     ``weight_out`` = ``pages.weight`` + share where that plane is given (used slots only)."""
     B, H = _check_query(q, c, pages)
     lib = _lib.load()
-    dev = q.device
+    dev = pages.device
     tp, tsb, mp = _table(pages, block_table, B)
-    _rows(lengths, (B,), "lengths", pages)
-    if accumulate and pages.weight is None:
-        raise ValueError("accumulate needs pages with a weight plane")
+    lp = _rows(lengths, (B,), "lengths", pages)
+    wo = None
+    if accumulate:
+        if pages.weight is None:
+            raise ValueError("accumulate needs pages with a weight plane")
+        wo = pages.weight if weight_out is None else weight_out
     if weight_out is not None:
         if not accumulate:
             raise ValueError("weight_out needs accumulate=True")
-        if tuple(weight_out.shape) != tuple(pages.weight.shape) or weight_out.stride() != pages.weight.stride() \
+        if weight_out.shape != pages.weight.shape or weight_out.stride() != pages.weight.stride() \
                 or weight_out.dtype != torch.float32 or weight_out.device != dev:
             raise ValueError("weight_out must be an fp32 plane with the shape and strides of pages.weight")
     if fgate is not None and pages.f is None:
         raise ValueError("fgate is given but the pages hold no f plane")
-    wo = None if not accumulate else (pages.weight if weight_out is None else weight_out)
+    for name, t in (("g", g), ("fgate", fgate)):
+        if t is not None and (t.numel() != B * H or t.device != dev):
+            raise ValueError(f"{name} must be ({B}, {H}, 1) on {dev}, got {tuple(t.shape)} on {t.device}")
+    if lam.shape != (H,) or lam.device != dev:
+        raise ValueError(f"lam must have shape {(H,)} on {dev}, got {tuple(lam.shape)} on {lam.device}")
     if c.dtype != q.dtype:
         c = c.to(q.dtype)
-    q, c = _operand(q), _operand(c)
-    gq = g.reshape(B, H).float().contiguous()
-    fq = None if fgate is None else fgate.reshape(B, H).float().contiguous()
-    lam = lam.float().contiguous()
-    if lam.shape != (H,):
-        raise ValueError(f"lam must have shape {(H,)}, got {tuple(lam.shape)}")
+    q, c, gq, lam = _operand(q), _operand(c), _f32(g), _f32(lam)
+    fq = None if fgate is None else _f32(fgate)
     y = torch.empty((B, H, 1, 64), device=dev, dtype=q.dtype)
     lse = torch.empty((B, H), device=dev, dtype=torch.float32) if return_lse else None
-    nbytes = lib.sisa_paged_attn_workspace(B, H, mp * pages.page_size, int(accumulate))
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    st = backends.status_word(dev)
-    vq, vc, vy = _lib.view4(q), _lib.view4(c), _lib.view4(y)
-    rc = lib.sisa_paged_attn(_lib.vref(vq), _lib.vref(vc), gq.data_ptr(), _lib.ptr(fq), pages.cref(), tp, tsb, mp,
-                             lengths.data_ptr(), lam.data_ptr(), B, H, pages.dtype_code, _lib.vref(vy), _lib.ptr(lse),
-                             _lib.ptr(wo), ws.data_ptr(), st.data_ptr(), _lib.stream_ptr(dev))
+    ws = torch.empty(lib.sisa_paged_attn_workspace(B, H, mp * pages.page_size, accumulate), dtype=torch.uint8, device=dev)
+    rc = lib.sisa_paged_attn(_lib.view4_bytes(q), _lib.view4_bytes(c), gq.data_ptr(), None if fq is None else fq.data_ptr(),
+                             pages.cbytes, tp, tsb, mp, lp, lam.data_ptr(), B, H, pages.dtype_code, _lib.view4_bytes(y),
+                             None if lse is None else lse.data_ptr(), None if wo is None else wo.data_ptr(), ws.data_ptr(),
+                             backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_attn")
     backends.after_call(dev)
     return (y, lse) if return_lse else y
@@ -177,13 +186,13 @@ def paged_evict(pages: KeyPages, block_table: Tensor, position: Tensor, budget: 
     weigh the same; -1 while the sequence holds fewer than ``budget`` keys. Returns (B, H) int32."""
     B, H = block_table.shape[0], pages.n_head
     tp, tsb, mp = _table(pages, block_table, B)
-    _rows(position, (B,), "position", pages)
-    slots = torch.empty((B, H), dtype=torch.int32, device=pages.device)
-    st = backends.status_word(pages.device)
-    rc = _lib.load().sisa_paged_evict(pages.cref(), tp, tsb, mp, position.data_ptr(), B, H, int(budget), int(recent),
-                                      slots.data_ptr(), st.data_ptr(), _lib.stream_ptr(pages.device))
+    pp = _rows(position, (B,), "position", pages)
+    dev = pages.device
+    slots = torch.empty((B, H), dtype=torch.int32, device=dev)
+    rc = _lib.load().sisa_paged_evict(pages.cbytes, tp, tsb, mp, pp, B, H, int(budget), int(recent), slots.data_ptr(),
+                                      backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_evict")
-    backends.after_call(pages.device)
+    backends.after_call(dev)
     return slots
 
 
@@ -198,46 +207,50 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
     after the write, min(position + 1, budget), is stored for :func:`paged_attention`.
 
     Returns q (a view of proj's Q columns), c~ (B, H, 1, 32), g and F (B, H, 1) fp32 (F None without z)."""
-    lib = _lib.load()
-    H = pages.n_head
-    if proj.dim() != 3 or proj.shape[1] != 1 or proj.shape[2] < 273 * H:
-        raise ValueError(f"proj must be (B, 1, >= {273 * H}), got {tuple(proj.shape)}")
-    B, dev = proj.shape[0], pages.device
+    H, dev = pages.n_head, pages.device
+    shape = proj.shape
+    if len(shape) != 3 or shape[1] != 1 or shape[2] < 273 * H:
+        raise ValueError(f"proj must be (B, 1, >= {273 * H}), got {tuple(shape)}")
+    B, _, width = shape
     if proj.dtype != pages.dtype:
         raise TypeError(f"projection dtype {proj.dtype} differs from the pages' {pages.dtype}")
     if proj.device != dev:
         raise ValueError(f"proj is on {proj.device}, the pages on {dev}")
     tp, tsb, mp = _table(pages, block_table, B)
-    _rows(position, (B,), "position", pages)
-    if slots is not None:
-        _rows(slots, (B, H), "slots", pages)
-    if lengths is not None:
-        _rows(lengths, (B,), "lengths", pages)
-    for name, t in (("carry", carry), ("carry_out", carry_out)):
-        if t is not None and (tuple(t.shape) != (B, H, CARRY) or t.dtype != torch.float32 or not t.is_contiguous()
-                              or t.device != dev):
-            raise ValueError(f"{name} must be a contiguous {(B, H, CARRY)} fp32 tensor on {dev}, got {tuple(t.shape)} "
-                             f"{t.dtype} on {t.device}")
-    if z is not None and pages.f is None:
-        raise ValueError("z is given but the pages hold no f plane")
+    pp = _rows(position, (B,), "position", pages)
+    sp = None if slots is None else _rows(slots, (B, H), "slots", pages)
+    lp = None if lengths is None else _rows(lengths, (B,), "lengths", pages)
     co = carry if carry_out is None else carry_out
-    proj2 = proj.reshape(B, proj.shape[-1])
-    if proj2.stride(-1) != 1 or proj2.stride(0) % 8 or proj2.data_ptr() % 16:
-        proj2 = proj2.contiguous()
+    for t in (carry, co):
+        if t.shape != (B, H, CARRY) or t.dtype != torch.float32 or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"carry must be a contiguous {(B, H, CARRY)} fp32 tensor on {dev}, got {tuple(t.shape)} "
+                             f"{t.dtype} on {t.device}")
+    sb, _, sl = proj.stride()
+    if sl != 1 or proj.data_ptr() % 16 or (sb % 8 and B > 1):
+        proj = proj.contiguous()
+        sb = width
+        if B > 1 and sb % 8:                    # rows of odd width: q's rows are read in 16-byte units
+            wide = proj.new_empty((B, 1, -(-width // 8) * 8))
+            wide[..., :width] = proj
+            proj, sb = wide, wide.shape[2]
     c = torch.empty((B, H, 1, 32), dtype=proj.dtype, device=dev)
     g = torch.empty((B, H, 1), dtype=torch.float32, device=dev)
-    z2 = f = None
+    z2 = f = zp = fp = None
     if z is not None:
-        z2 = z.reshape(B, H).float().contiguous()
+        if pages.f is None:
+            raise ValueError("z is given but the pages hold no f plane")
+        if z.numel() != B * H or z.device != dev:
+            raise ValueError(f"z must be ({B}, 1, {H}) on {dev}, got {tuple(z.shape)} on {z.device}")
+        z2 = _f32(z)
         f = torch.empty((B, H, 1), dtype=torch.float32, device=dev)
-    st = backends.status_word(dev)
-    rc = lib.sisa_paged_append(proj2.data_ptr(), proj2.stride(0) if B > 1 else proj2.shape[1], _lib.ptr(z2), H,
-                               pages.cref(), tp, tsb, mp, position.data_ptr(), _lib.ptr(slots), int(budget or 0), B, H,
-                               pages.dtype_code, carry.data_ptr(), co.data_ptr(), c.data_ptr(), g.data_ptr(),
-                               _lib.ptr(f), _lib.ptr(lengths), st.data_ptr(), _lib.stream_ptr(dev))
+        zp, fp = z2.data_ptr(), f.data_ptr()
+    rc = _lib.load().sisa_paged_append(proj.data_ptr(), sb if B > 1 else width, zp, H, pages.cbytes, tp, tsb, mp, pp, sp,
+                                       int(budget or 0), B, H, pages.dtype_code, carry.data_ptr(), co.data_ptr(),
+                                       c.data_ptr(), g.data_ptr(), fp, lp, backends.status_word(dev).data_ptr(),
+                                       _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_append")
     backends.after_call(dev)
-    return proj2[:, :H * 64].view(B, H, 64).unsqueeze(2), c, g, f
+    return proj.as_strided((B, H, 1, 64), (sb, 64, 64, 1)), c, g, f
 
 
 def attention_key_weights(q: Tensor, k: Tensor, c: Tensor, b: Tensor, pos: Tensor, lam: Tensor, lse: Tensor, *,
@@ -249,17 +262,17 @@ def attention_key_weights(q: Tensor, k: Tensor, c: Tensor, b: Tensor, pos: Tenso
     if q.dim() != 4 or q.shape[-1] != 64:
         raise ValueError(f"q must be (B, H, L, 64), got {tuple(q.shape)}")
     B, H, L, _ = q.shape
-    if tuple(k.shape) != (B, H, L, 64) or tuple(c.shape) != (B, H, L, 32) or tuple(b.shape) != (B, H, L, 32):
+    if k.shape != (B, H, L, 64) or c.shape != (B, H, L, 32) or b.shape != (B, H, L, 32):
         raise ValueError(f"k, c and b must be {(B, H, L, 64)}, {(B, H, L, 32)} and {(B, H, L, 32)}, got "
                          f"{tuple(k.shape)}, {tuple(c.shape)} and {tuple(b.shape)}")
     if any(t.dtype != q.dtype for t in (k, c, b)):
         raise TypeError(f"q, k, c and b differ in dtype: {q.dtype}, {k.dtype}, {c.dtype}, {b.dtype}")
     lib = _lib.load()
     code = _lib.dtype_code(q.dtype)
-    if tuple(pos.shape) != (B, H, 4, lib.sisa_pos_len(L)) or not pos.is_contiguous() or pos.dtype != torch.float32:
+    if pos.shape != (B, H, 4, lib.sisa_pos_len(L)) or not pos.is_contiguous() or pos.dtype != torch.float32:
         raise ValueError(f"pos must be the contiguous position planes {(B, H, 4, lib.sisa_pos_len(L))}, got "
                          f"{tuple(pos.shape)} {pos.dtype}")
-    if tuple(lse.shape) != (B, H, L) or lse.dtype != torch.float32:
+    if lse.shape != (B, H, L) or lse.dtype != torch.float32:
         raise ValueError(f"lse must be {(B, H, L)} fp32, got {tuple(lse.shape)} {lse.dtype}")
     lam = lam.float().contiguous()
     if lam.shape != (H,):
@@ -269,10 +282,9 @@ def attention_key_weights(q: Tensor, k: Tensor, c: Tensor, b: Tensor, pos: Tenso
         raise ValueError("attention_key_weights takes CUDA tensors on one device")
     q, k, c, b, lse = _operand(q), _operand(k), _operand(c), _operand(b), lse.contiguous()
     w = torch.empty((B, H, L), dtype=torch.float32, device=dev)
-    st = backends.status_word(dev)
-    vs = [_lib.view4(t) for t in (q, k, c, b)]
-    rc = lib.sisa_attn_key_weights(*(_lib.vref(v) for v in vs), pos.data_ptr(), lam.data_ptr(), lse.data_ptr(), B, H, L,
-                                   int(first_query), code, w.data_ptr(), st.data_ptr(), _lib.stream_ptr(dev))
+    rc = lib.sisa_attn_key_weights(*map(_lib.view4_bytes, (q, k, c, b)), pos.data_ptr(), lam.data_ptr(), lse.data_ptr(), B,
+                                   H, L, int(first_query), code, w.data_ptr(), backends.status_word(dev).data_ptr(),
+                                   _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_attn_key_weights")
     backends.after_call(dev)
     return w
@@ -310,12 +322,10 @@ def paged_fill(pages: KeyPages, block_table: Tensor, k: Tensor, v: Tensor, b: Te
     lib = _lib.load()
     ws = torch.empty(max(lib.sisa_paged_fill_workspace(B, H, keep), 16), dtype=torch.uint8, device=dev)
     k, v, b = _operand(k), _operand(v), _operand(b)
-    vk, vv, vb = _lib.view4(k), _lib.view4(v), _lib.view4(b)
     fs = (0, 0) if fgate is None else fgate.stride()[:2]
-    st = backends.status_word(dev)
-    rc = lib.sisa_paged_fill(pages.cref(), tp, tsb, mp, _lib.vref(vk), _lib.vref(vv), _lib.vref(vb), g.data_ptr(),
-                             g.stride(0), g.stride(1), _lib.ptr(fgate), *fs, _lib.ptr(weight), B, H, L, keep, int(recent),
-                             ws.data_ptr(), st.data_ptr(), _lib.stream_ptr(dev))
+    rc = lib.sisa_paged_fill(pages.cbytes, tp, tsb, mp, *map(_lib.view4_bytes, (k, v, b)), g.data_ptr(), g.stride(0),
+                             g.stride(1), _lib.ptr(fgate), *fs, _lib.ptr(weight), B, H, L, keep, int(recent), ws.data_ptr(),
+                             backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_fill")
     backends.after_call(dev)
     return keep
