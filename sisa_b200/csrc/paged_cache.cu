@@ -12,41 +12,91 @@ namespace pca {
 
 constexpr int NT = 256, NW = NT / 32;
 
+__device__ __forceinline__ int cluster_blocks() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return (int)n;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+}
+// The 64-bit word of block `rank` of this cluster at the shared-memory place of `p`.
+__device__ __forceinline__ unsigned long long cluster_load(const unsigned long long* p, int rank) {
+  uint32_t addr;
+  unsigned long long v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // ------------------------------------------------------------------------------------ evict
-// One block per (batch, head): slots[b, h] = the slot j < budget of the least weight among the keys whose
-// token is older than the `recent` newest (token < position - recent), the lowest slot where several
-// weigh the same; -1 while the sequence holds fewer than budget keys. (weight, slot) is one 64-bit key,
-// so the minimum does not depend on the order in which it is taken.
+// slots[b, h] = the slot j < budget of the least weight among the keys whose token is older than the `recent`
+// newest (token < position - recent), the lowest slot where several weigh the same; -1 while the sequence
+// holds fewer than budget keys. (weight, slot) is one 64-bit number, so the minimum does not depend on the
+// order in which it is taken.
+// HBM-bound: 8 bytes per key. A thread takes four slots at a time (16-byte loads of both planes), two such
+// steps in flight; a cluster of blocks shares a unit when there are few units, and its first block takes
+// the minimum over the others' through distributed shared memory.
+constexpr int EVICT_CLUSTER = 8;                 // portable cluster size
 __global__ void __launch_bounds__(NT) paged_evict_kernel(PagedEvictParams p) {
-  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, tid = threadIdx.x;
+  const int cs = cluster_blocks(), rank = blockIdx.x % cs;
+  const int bh = blockIdx.x / cs, b = bh / p.H, h = bh % p.H, tid = threadIdx.x;
   const int64_t pos = p.position[b];
-  if (pos < p.budget) {
-    if (tid == 0) p.slots[bh] = -1;
-    return;
-  }
-  const int64_t newest = pos - p.recent;
+  __shared__ unsigned long long s_best[NW + 1];
   unsigned long long best = ~0ull;
-  for (int64_t j = tid; j < p.budget; j += NT) {
-    const int page = page_of(p.pg, b, j, p.status);
-    if (page < 0) continue;
-    const int64_t at = page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
-    if (p.pg.token[at] >= newest) continue;
-    const unsigned long long key = ((unsigned long long)weight_order(p.pg.weight[at]) << 32) | (unsigned)j;
-    best = key < best ? key : best;
-  }
+  if (pos >= p.budget) {                         // uniform over the cluster
+    const int64_t newest = pos - p.recent;
+    const int64_t step = (int64_t)cs * NT * 4;
+    struct Four { float4 w; int4 t; bool ok; };
+    auto load = [&](int64_t j) {
+      Four f;
+      f.ok = false;
+      if (j >= p.budget) return f;
+      const int page = page_of(p.pg, b, j, p.status);
+      if (page < 0) return f;
+      const int64_t at = page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
+      f.w = __ldg(reinterpret_cast<const float4*>(p.pg.weight + at));
+      f.t = __ldg(reinterpret_cast<const int4*>(p.pg.token + at));
+      f.ok = true;
+      return f;
+    };
+    auto take = [&](const Four& f, int64_t j) {
+      if (!f.ok) return;
+      const float w[4] = {f.w.x, f.w.y, f.w.z, f.w.w};
+      const int t[4] = {f.t.x, f.t.y, f.t.z, f.t.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-    best = other < best ? other : best;
+      for (int e = 0; e < 4; ++e) {
+        const unsigned long long key = ((unsigned long long)weight_order(w[e]) << 32) | (unsigned)(j + e);
+        if (j + e < p.budget && t[e] < newest && key < best) best = key;
+      }
+    };
+    for (int64_t j = ((int64_t)rank * NT + tid) * 4; j < p.budget; j += 2 * step) {
+      const Four f0 = load(j), f1 = load(j + step);
+      take(f0, j);
+      take(f1, j + step);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+      best = other < best ? other : best;
+    }
+    if ((tid & 31) == 0) s_best[tid >> 5] = best;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < NW; ++w) best = s_best[w] < best ? s_best[w] : best;
+      s_best[NW] = best;
+    }
   }
-  __shared__ unsigned long long s_best[NW];
-  if ((tid & 31) == 0) s_best[tid >> 5] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < NW; ++w) best = s_best[w] < best ? s_best[w] : best;
+  if (cs > 1) cluster_sync();
+  if (rank == 0 && tid == 0) {
+    for (int r = 1; r < cs && pos >= p.budget; ++r) {
+      const unsigned long long other = cluster_load(&s_best[NW], r);
+      best = other < best ? other : best;
+    }
     p.slots[bh] = best == ~0ull ? -1 : (int)(unsigned)best;
-    if (best == ~0ull && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
+    if (pos >= p.budget && best == ~0ull && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
   }
+  if (cs > 1) cluster_sync();                    // the others' shared memory stays until it has been read
 }
 
 // ------------------------------------------------------------------------------------ append
@@ -129,10 +179,19 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) 
 
 // ------------------------------------------------------------------------------------ fill
 // The kept keys of one (batch, head), ascending: the last `recent`, and of the rest the keep - recent of
-// the largest weight, the earlier position where two weigh the same. A radix select over the ordered
-// weights (eight bits a pass) finds the smallest kept weight T and how many of the keys at T are kept;
-// a block scan then writes the kept positions in order.
-__device__ __forceinline__ int block_scan_excl(int v, int* s_warp, int& total) {
+// the largest weight, the earlier position where two weigh the same. One block per unit:
+//   1. a radix select over the ordered weights (11 + 11 + 10 bits) finds the smallest kept weight T and how
+//      many of the keys at T are kept;
+//   2. per 32-key group the kept keys above T and the ties are counted, two block scans (ties first: how
+//      many of them a group keeps depends on those before it) place the groups, and the kept positions
+//      are written in order.
+// The weights of up to SEL_SMEM keys are ordered once into shared memory; longer prompts are read again
+// from L2 in each pass. With it and 1024 threads a unit of 8192 keys takes about 10 us.
+constexpr int ST = 1024, SEL_SMEM = 40960;
+constexpr int BINS = 2048;
+
+// Exclusive scan over the block's threads; total in every thread.
+__device__ __forceinline__ int scan_excl(int v, int* s_warp, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
 #pragma unroll
@@ -142,99 +201,177 @@ __device__ __forceinline__ int block_scan_excl(int v, int* s_warp, int& total) {
   }
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
-  int base = 0;
-  total = 0;
+  const int c = s_warp[lane];                    // ST / 32 == 32 warps
+  int y = c;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const int c = s_warp[w];
-    if (w < warp) base += c;
-    total += c;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
   }
+  total = __shfl_sync(0xffffffffu, y, 31);
+  const int base = __shfl_sync(0xffffffffu, y - c, warp);
   __syncthreads();
   return base + x - v;
 }
 
-__global__ void __launch_bounds__(NT) paged_select_kernel(PagedFillParams p) {
-  const int bh = blockIdx.x, tid = threadIdx.x;
+__global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
+  extern __shared__ uint32_t s_key[];            // ordered weights of positions [0, old) when they fit
+  __shared__ int s_hist[BINS], s_warp[32], s_base[ST], s_tie[ST];
+  __shared__ uint32_t s_digit;
+  __shared__ int s_left;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int32_t* out = p.index + (int64_t)bh * p.keep;
-  const float* wt = p.weight ? p.weight + (int64_t)bh * p.L : nullptr;
-  const int64_t old = p.L - p.recent;              // positions [0, old) compete for keep - recent places
-  __shared__ int s_hist[256], s_warp[NW];
-  __shared__ uint32_t s_prefix;
-  __shared__ int64_t s_left;
+  const int L = (int)p.L, old = (int)(p.L - p.recent);   // positions [0, old) compete for keep - recent places
+  const bool all = p.keep == p.L;
+  if (all) {
+    for (int j = tid; j < L; j += ST) out[j] = j;
+    return;
+  }
+  const float* wt = p.weight + (int64_t)bh * p.L;
+  const bool in_smem = old <= SEL_SMEM;
+  if (in_smem) {
+    for (int j = tid; j < old; j += ST) s_key[j] = weight_order(__ldg(wt + j));
+  }
+  __syncthreads();
+  auto key_at = [&](int j) { return in_smem ? s_key[j] : weight_order(__ldg(wt + j)); };
   uint32_t prefix = 0;
-  int64_t left = p.keep - p.recent;                // places left among the keys that match the prefix
-  if (wt && p.keep < p.L) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      s_hist[tid] = 0;
+  int left = (int)(p.keep - p.recent);           // places left among the keys that match the prefix
+  if (left > 0) {
+    int shift = 32;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int bits = pass < 2 ? 11 : 10, above = shift;
+      shift -= bits;
+      for (int i = tid; i < BINS; i += ST) s_hist[i] = 0;
       __syncthreads();
-      for (int64_t j = tid; j < old; j += NT) {
-        const uint32_t u = weight_order(wt[j]);
-        if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(u >> shift) & 255], 1);
+      for (int j = tid; j < old; j += ST) {
+        const uint32_t u = key_at(j);
+        if (above == 32 || (u >> above) == (prefix >> above)) atomicAdd(&s_hist[(u >> shift) & ((1u << bits) - 1)], 1);
       }
       __syncthreads();
-      if (tid == 0) {
-        int64_t n = left;
-        int d = 255;
-        while (d > 0 && n > s_hist[d]) n -= s_hist[d--];
-        s_prefix = prefix | ((uint32_t)d << shift);
-        s_left = n;
-      }
+      // thread t holds the bins 2047 - 2t and 2046 - 2t: the scan runs from the largest digit down
+      const int d = BINS - 1 - 2 * tid, h0 = s_hist[d], h1 = s_hist[d - 1];
+      int total;
+      const int over = scan_excl(h0 + h1, s_warp, total);
+      if (over < left && left <= over + h0) { s_digit = d; s_left = left - over; }
+      else if (over + h0 < left && left <= over + h0 + h1) { s_digit = d - 1; s_left = left - over - h0; }
       __syncthreads();
-      prefix = s_prefix;
+      prefix |= s_digit << shift;
       left = s_left;
       __syncthreads();
     }
   }
-  const bool all = !wt || p.keep == p.L;
-  int64_t done = 0, ties = 0;                       // kept so far, keys at the threshold so far
-  for (int64_t j0 = 0; j0 < p.L; j0 += NT) {
-    const int64_t j = j0 + tid;
-    const uint32_t u = (!all && j < old) ? weight_order(wt[j]) : 0u;
-    const bool tie = !all && j < old && u == prefix;
-    int tot = 0, rank = 0;
-    if (!all) {
-      rank = block_scan_excl(tie ? 1 : 0, s_warp, tot);
+  // with left == 0 nothing but the newest is kept: no key is above the largest order
+  if (p.keep == p.recent) prefix = 0xffffffffu;
+  int done = 0, ties = 0;                        // kept, and keys at T, in the chunks before
+  for (int j0 = 0; j0 < L; j0 += ST * 32) {
+    // group (warp + 32 i) of the chunk holds 32 consecutive positions
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      const int g = warp + 32 * i, j = j0 + g * 32 + lane;
+      if (j0 + g * 32 >= L) {
+        if (lane == 0) { s_base[g] = 0; s_tie[g] = 0; }
+        continue;
+      }
+      const uint32_t u = j < old ? key_at(j) : 0u;
+      const uint32_t sure = __ballot_sync(0xffffffffu, j < L && (j >= old || u > prefix));
+      const uint32_t tie = __ballot_sync(0xffffffffu, j < old && u == prefix);
+      if (lane == 0) { s_base[g] = __popc(sure); s_tie[g] = __popc(tie); }
     }
-    const bool keep = j < p.L && (all || j >= old || u > prefix || (tie && ties + rank < left));
-    int kept;
-    const int at = block_scan_excl(keep ? 1 : 0, s_warp, kept);
-    if (keep && done + at < p.keep) out[done + at] = (int)j;
-    done += kept;
-    ties += tot;
+    __syncthreads();
+    int tot_tie, tot;
+    const int nt = s_tie[tid], ns = s_base[tid];
+    const int tb = ties + scan_excl(nt, s_warp, tot_tie);
+    const int mine = ns + max(0, min(nt, left - tb));
+    const int at = done + scan_excl(mine, s_warp, tot);
+    s_base[tid] = at;
+    s_tie[tid] = tb;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      const int g = warp + 32 * i, j = j0 + g * 32 + lane;
+      if (j0 + g * 32 >= L) break;
+      const uint32_t u = j < old ? key_at(j) : 0u;
+      const bool tie = j < old && u == prefix;
+      const uint32_t below = (1u << lane) - 1, ties_in = __ballot_sync(0xffffffffu, tie);
+      const bool keep = j < L && (j >= old || u > prefix || (tie && s_tie[g] + __popc(ties_in & below) < left));
+      const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+      if (keep) out[s_base[g] + __popc(kept & below)] = j;
+    }
+    __syncthreads();
+    done += tot;
+    ties += tot_tie;
   }
 }
 
-// Eight lanes per kept key copy its rows (16 bytes a lane) and its plane values into slot r of the
-// sequence's pages.
+// 64 kept keys of one unit per block: eight lanes per key copy its rows (16 bytes a lane, two keys a lane so
+// that six loads are in flight), 64 threads its plane values, into the sequence's pages.
+constexpr int GK = 64;
 __global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
-  const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H;
-  const int64_t r = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  const int part = threadIdx.x & 7;
-  if (r >= p.keep) return;
-  const int64_t j = p.index[(int64_t)bh * p.keep + r];
-  const int page = page_of(p.pg, b, r, p.status);
-  if (page < 0) return;
-  const int64_t in = r & ((1 << p.pg.page_shift) - 1);
-  reinterpret_cast<uint4*>(p.pg.k + 2 * (page * p.pg.k_sp + h * p.pg.k_sh + in * 64))[part] =
-      reinterpret_cast<const uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + j * p.k_sl))[part];
-  reinterpret_cast<uint4*>(p.pg.v + 2 * (page * p.pg.v_sp + h * p.pg.v_sh + in * 64))[part] =
-      reinterpret_cast<const uint4*>(p.v + 2 * (b * p.v_sb + h * p.v_sh + j * p.v_sl))[part];
-  if (part < 4)
-    reinterpret_cast<uint4*>(p.pg.b + 2 * (page * p.pg.b_sp + h * p.pg.b_sh + in * 32))[part] =
-        reinterpret_cast<const uint4*>(p.b + 2 * (b * p.b_sb + h * p.b_sh + j * p.b_sl))[part];
-  const int64_t at = page * p.pg.s_sp + h * p.pg.s_sh + in;
-  if (part == 4) p.pg.g[at] = p.g[b * p.g_sb + h * p.g_sh + j];
-  if (part == 5 && p.pg.f) p.pg.f[at] = p.f ? p.f[b * p.f_sb + h * p.f_sh + j] : 0.f;
-  if (part == 6 && p.pg.weight) p.pg.weight[at] = p.weight ? p.weight[(int64_t)bh * p.L + j] : 0.f;
-  if (part == 7 && p.pg.token) p.pg.token[at] = (int)j;
+  const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H, tid = threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * GK;
+  const int part = tid & 7;
+  const int32_t* index = p.index + (int64_t)bh * p.keep;
+  int pages[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = r0 + i * 32 + (tid >> 3);
+    pages[i] = r < p.keep ? page_of(p.pg, b, r, p.status) : -1;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  uint4 k[2], v[2], m[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = r0 + i * 32 + (tid >> 3);
+    if (pages[i] < 0) continue;
+    const int64_t j = index[r];
+    k[i] = __ldg(reinterpret_cast<const uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + j * p.k_sl)) + part);
+    v[i] = __ldg(reinterpret_cast<const uint4*>(p.v + 2 * (b * p.v_sb + h * p.v_sh + j * p.v_sl)) + part);
+    if (part < 4) m[i] = __ldg(reinterpret_cast<const uint4*>(p.b + 2 * (b * p.b_sb + h * p.b_sh + j * p.b_sl)) + part);
+  }
+  if (tid < GK && r0 + tid < p.keep) {
+    const int64_t r = r0 + tid, j = index[r];
+    const int page = page_of(p.pg, b, r, nullptr);
+    if (page >= 0) {
+      const int64_t at = page * p.pg.s_sp + h * p.pg.s_sh + (r & ((1 << p.pg.page_shift) - 1));
+      const float g = __ldg(p.g + b * p.g_sb + h * p.g_sh + j);
+      const float f = p.f ? __ldg(p.f + b * p.f_sb + h * p.f_sh + j) : 0.f;
+      const float w = p.weight ? __ldg(p.weight + (int64_t)bh * p.L + j) : 0.f;
+      p.pg.g[at] = g;
+      if (p.pg.f) p.pg.f[at] = f;
+      if (p.pg.weight) p.pg.weight[at] = w;
+      if (p.pg.token) p.pg.token[at] = (int)j;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t in = (r0 + i * 32 + (tid >> 3)) & ((1 << p.pg.page_shift) - 1), page = pages[i];
+    if (page < 0) continue;
+    reinterpret_cast<uint4*>(p.pg.k + 2 * (page * p.pg.k_sp + h * p.pg.k_sh + in * 64))[part] = k[i];
+    reinterpret_cast<uint4*>(p.pg.v + 2 * (page * p.pg.v_sp + h * p.pg.v_sh + in * 64))[part] = v[i];
+    if (part < 4) reinterpret_cast<uint4*>(p.pg.b + 2 * (page * p.pg.b_sp + h * p.pg.b_sh + in * 32))[part] = m[i];
+  }
 }
 
 }  // namespace pca
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, cudaStream_t st) {
-  pca::paged_evict_kernel<<<p.B * p.H, pca::NT, 0, st>>>(p);
-  return cudaGetLastError();
+  // blocks per unit: enough for four blocks per SM, each with at least one step of 1024 slots
+  const int64_t units = (int64_t)p.B * p.H;
+  int cs = 1;
+  while (cs < pca::EVICT_CLUSTER && units * cs < 148 * 4 && (int64_t)cs * pca::NT * 4 < p.budget) cs *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(units * cs));
+  cfg.blockDim = dim3(pca::NT);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, pca::paged_evict_kernel, p);
 }
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, cudaStream_t st) {
@@ -245,10 +382,23 @@ cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, cudaStrea
 }
 
 cudaError_t launch_paged_fill(const PagedFillParams& p, cudaStream_t st) {
-  pca::paged_select_kernel<<<p.B * p.H, pca::NT, 0, st>>>(p);
-  dim3 grid((unsigned)((p.keep + 31) / 32), p.B * p.H);
-  pca::paged_gather_kernel<<<grid, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  const int64_t old = p.L - p.recent;
+  const size_t smem = p.keep < p.L && old <= pca::SEL_SMEM ? (size_t)old * 4 : 0;
+  cudaError_t e = cudaFuncSetAttribute(pca::paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       pca::SEL_SMEM * 4);
+  if (e != cudaSuccess) return e;
+  pca::paged_select_kernel<<<p.B * p.H, pca::ST, smem, st>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((p.keep + pca::GK - 1) / pca::GK), p.B * p.H);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its blocks wait for the choice themselves
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, pca::paged_gather_kernel, p);
 }
 
 }  // namespace sisa
