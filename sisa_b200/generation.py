@@ -182,7 +182,10 @@ class DecodeGraph:
         first = next(model.parameters())
         dev = first.device
         self.cache = cache
-        self.states = [cache.get(i) for i in range(len(model.layers))]
+        self.paged = getattr(cache, "paged", False)     # a PagedCache keeps its counters on the device itself
+        if self.paged and cache.count != batch:
+            raise ValueError(f"DecodeGraph: the paged cache has {cache.count} rows, the batch {batch}")
+        self.states = [] if self.paged else [cache.get(i) for i in range(len(model.layers))]
         self.stream = stream if stream is not None else torch.cuda.Stream(dev)   # capture (and replay) stream
         self.ids = torch.zeros((batch, 1), dtype=torch.long, device=dev)
         self.pos_dev = torch.full((1,), cache.seq_len, dtype=torch.int32, device=dev)
@@ -190,6 +193,8 @@ class DecodeGraph:
         for st in self.states:
             st.phi_buffer()
             st.pos_dev = self.pos_dev
+        if self.paged:
+            cache.before_step()
         self.graph = torch.cuda.CUDAGraph()
         self.stream.wait_stream(torch.cuda.current_stream(dev))
         try:
@@ -222,6 +227,8 @@ class DecodeGraph:
 
     def room(self) -> int:
         """Steps left before the cache is full."""
+        if self.paged:
+            return self.cache.room()
         return min(st.capacity - st.length for st in self.states)
 
     def step(self, ids: Tensor) -> Tensor:
@@ -230,6 +237,11 @@ class DecodeGraph:
         if self.room() < 1:
             raise ValueError("DecodeGraph: the cache is full")
         self.ids.copy_(ids.reshape(-1, 1))
+        if self.paged:
+            self.cache.before_step()             # pages for the new tokens: the table is read by the captured step
+            self.graph.replay()
+            self.cache.advance_host()
+            return self.logits
         self.graph.replay()
         for st in self.states:
             st.length += 1
@@ -301,7 +313,9 @@ def _check_generate_args(input_ids: Tensor, max_new_tokens: int, do_sample: bool
 def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, temperature: float = 1.0,
              top_k: int | None = None, eos_token_id: int | Iterable[int] | Tensor | None = None,
              do_sample: bool = False, *, generator: torch.Generator | None = None,
-             eos_check_every: int = 16, cuda_graph: bool = True) -> Tensor:
+             eos_check_every: int = 16, cuda_graph: bool = True, page_size: int | None = None,
+             cache_budget: int | None = None, cache_recent: int | None = None,
+             cache_observe: int | None = None) -> Tensor:
     """Generate continuations of ``input_ids`` (generation.py:139-191).
 
     Same results as the reference. The all-finished check reads the device only every
@@ -309,6 +323,12 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
     cut off afterwards, so the returned length is the reference's. With ``cuda_graph`` (default) and a
     model that :meth:`DecodeGraph.supported` accepts, the first decode step runs eagerly and the rest
     replay it as one CUDA graph.
+
+    With ``page_size`` or ``cache_budget`` (no counterpart in the reference) the keys lie in a
+    :class:`~sisa_b200.paged_cache.PagedCache` (cuda path only). ``cache_budget`` bounds the keys kept per
+    head and sequence: of the prompt the ``cache_recent`` newest (default a quarter) and those that received
+    most attention from its last ``cache_observe`` queries (default all), then every new token replaces the
+    least attended old key. Without a budget, or with one that is never reached, nothing is dropped.
     """
     _check_generate_args(input_ids, max_new_tokens, do_sample, temperature, top_k)
     squeeze = input_ids.dim() == 1
@@ -318,7 +338,12 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
         return input_ids.squeeze(0) if squeeze else input_ids
     eos = _eos_ids(eos_token_id)
     eos_t = torch.tensor(eos, device=input_ids.device, dtype=input_ids.dtype) if eos else None
-    cache = SISACache(capacity=input_ids.shape[1] + max_new_tokens)
+    total = input_ids.shape[1] + max_new_tokens
+    cache = SISACache(capacity=total)
+    if page_size is not None or cache_budget is not None:
+        cache = _paged_cache(model, input_ids, total, page_size, cache_budget, cache_recent, cache_observe)
+    elif cache_recent is not None or cache_observe is not None:
+        raise ValueError("cache_recent and cache_observe need cache_budget")
     logits = model(input_ids, cache=cache, logits_to_keep=1).logits[:, -1]
     pieces = [input_ids]
     done = torch.zeros(input_ids.shape[0], dtype=torch.bool, device=input_ids.device)
@@ -332,6 +357,19 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
         if hit.numel():
             out = out[:, :input_ids.shape[1] + int(hit[0]) + 1]
     return out.squeeze(0) if squeeze else out
+
+
+def _paged_cache(model, input_ids, total, page_size, budget, recent, observe):
+    """The paged cache of :func:`generate` (raises where the cuda path cannot run)."""
+    from .modeling import _compute_dtype, _resolve_impl
+    from .paged_cache import PagedCache
+
+    probe = model.embed.weight[:1].detach().unsqueeze(0)
+    if not probe.is_cuda or _resolve_impl(model.config.attn_impl, probe, model.config) != "cuda":
+        raise ValueError("page_size and cache_budget need the model on the cuda attention path")
+    return PagedCache(model.config, input_ids.shape[0], max_tokens=total if budget is None else None, budget=budget,
+                      recent=recent, observe=observe, page_size=64 if page_size is None else page_size,
+                      dtype=_compute_dtype(probe), device=probe.device)
 
 
 def _decode_loop(model, input_ids, max_new_tokens, logits, cache, pieces, done, all_done_at, eos_t, do_sample,

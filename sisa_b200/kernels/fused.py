@@ -189,7 +189,8 @@ class _SISAFusedFn(torch.autograd.Function):
         return dproj, (dz if z is not None else None), dlam, None
 
 
-def prefill_layer(proj: torch.Tensor, z: torch.Tensor, lam: torch.Tensor, n_head: int):
+def prefill_layer(proj: torch.Tensor, z: torch.Tensor, lam: torch.Tensor, n_head: int,
+                  weigh_from: int | None = None):
     """The layer core over a whole prompt without autograd, keeping what a decode cache needs: the
     preparation kernel and the tcgen05 forward (no o'' - nothing will run a backward), on the fused
     projection ``proj`` (B, L, NPAD) and forget logits ``z`` (B, L, H) fp32.
@@ -197,17 +198,24 @@ def prefill_layer(proj: torch.Tensor, z: torch.Tensor, lam: torch.Tensor, n_head
     The reference fills its cache through the unfused path instead (src/sisa/modeling.py:226-232: seven
     projections, torch recurrences and rotations). Returns ``y`` (B, L, H*64) and the cache entries:
     k, v (views of proj's K/V columns), b~ (B, H, L, 32) as the kernels rotated it, g and F (views of the
-    position planes) and Phi at the last position (B, H, 16) fp32."""
+    position planes) and Phi at the last position (B, H, 16) fp32. With ``weigh_from`` a seventh entry holds the
+    attention each key received from the queries at and after that position (B, H, L) fp32, for a cache that
+    keeps only the heaviest keys."""
     H = int(n_head)
     B, L, _ = proj.shape
     off = fused_layout(H)
     c_rot, b_rot, pos, _ = ops.prep_fwd(proj, z, H)
     q, k, v = ops.heads(proj, off["Q"], H, 64), ops.heads(proj, off["K"], H, 64), ops.heads(proj, off["V"], H, 64)
-    o, _, _ = ops.attn_fwd(q, k, v, c_rot, b_rot, pos, lam, False)
+    o, lse, _ = ops.attn_fwd(q, k, v, c_rot, b_rot, pos, lam, False)
+    extra = ()
+    if weigh_from is not None:
+        from .paged import attention_key_weights
+
+        extra = (attention_key_weights(q, k, c_rot, b_rot, pos, lam, lse, first_query=weigh_from),)
     theta = proj[..., off["TH"]:off["TH"] + H * (D_STATE // 2)]
     phi_last = theta.float().sum(dim=1).view(B, H, D_STATE // 2)
     y = o.transpose(1, 2).reshape(B, L, H * D_HEAD)
-    return y, (k, v, b_rot, pos[:, :, 0, :L], pos[:, :, 1, :L], phi_last)
+    return y, (k, v, b_rot, pos[:, :, 0, :L], pos[:, :, 1, :L], phi_last) + extra
 
 
 def sisa_fused(proj: torch.Tensor, z: torch.Tensor | None, lam: torch.Tensor, n_head: int) -> torch.Tensor:

@@ -315,8 +315,11 @@ class SISAAttention(nn.Module):
 
         weight, bias = self._fused_weights_static()
         proj = F.linear(x, weight, bias)
-        q, c, g, fgate = decode_prep(proj, self._forget_logits(x) if z is None else z, state, self.config.n_head)
+        z = self._forget_logits(x) if z is None else z
         lam = _static(self, "_lam_static", lambda t: F.softplus(t).float(), self.lambda_raw)
+        if getattr(state, "paged", False):       # rows of a PagedCache: slot choice, append and attention on pages
+            return self._output(state.step(proj, z, lam))
+        q, c, g, fgate = decode_prep(proj, z, state, self.config.n_head)
         return self._output(decode_attention(q, c, g, fgate, state, lam))
 
     def _prefill_fused(self, x: Tensor, cache: "SISACache", z: Tensor | None = None) -> Tensor:
@@ -329,8 +332,13 @@ class SISAAttention(nn.Module):
         weight, bias = self._fused_weights_static()
         proj = F.linear(x, weight, bias)
         lam = _static(self, "_lam_static", lambda t: F.softplus(t).float(), self.lambda_raw)
-        y, (k, v, b, g, fgate, phi) = prefill_layer(proj, self._forget_logits(x) if z is None else z, lam,
-                                                     self.config.n_head)
+        z = self._forget_logits(x) if z is None else z
+        if getattr(cache, "paged", False):
+            first = cache.weigh_from(x.shape[1])
+            y, entries = prefill_layer(proj, z, lam, self.config.n_head, weigh_from=first)
+            cache.fill(self.layer_idx, *entries, *(() if first is not None else (None,)))
+            return self.W_O(y)
+        y, (k, v, b, g, fgate, phi) = prefill_layer(proj, z, lam, self.config.n_head)
         cache.update(self.layer_idx, k=k, v=v, b=b, g=g, fgate=fgate, phi=phi)
         return self.W_O(y)
 
@@ -352,6 +360,9 @@ class SISAAttention(nn.Module):
             return self._decode_fused(x, state)
         if self._use_fused_prefill(x, state, requested):
             return self._prefill_fused(x, cache)
+        if getattr(cache, "paged", False):
+            raise ValueError("a paged cache takes a prompt into empty rows, then one token per row, on the cuda attention "
+                             "path without autograd, in its own dtype")
         q, k, v, c, b, g, fgate, phi = self._prepare(x, state)
         if state is None:
             impl = _resolve_impl(requested, x, self.config)
