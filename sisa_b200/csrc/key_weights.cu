@@ -7,17 +7,17 @@
 // first) to the end. Warp roles:
 //   warps 0-7  compute: a thread owns one key row (TMEM lane) and 32 of a tile's 64 query columns, so the
 //              sum over queries is thread-local and the two halves meet once at the end,
-//   warp 8     TMA producer of the Q, C and position tiles; its lanes also bring the tile's lse values,
+//   warp 8     TMA producer of the Q, C and position tiles; its lanes also form the queries' additive terms,
 //   warp 9     UMMA issuer and TMEM owner.
 // Per tile S^T = K Q^T (M128 N64 K64) and U^T = B~ C^T (K32) land in one of two TMEM buffers, so the next
 // tile's GEMMs run under this tile's arithmetic; two CTAs share an SM (2 x 256 TMEM columns).
 // Off the diagonal the decay is the product of three factors <= 1: the query's within its 64-row block (a
 // stored plane), the one between the blocks (one per tile) and the key's to the end of its tile (one per
-// thread). F_i - F_j is taken before the log2e scaling. Per element that leaves 3 packed-fp32 issue slots
-// and one exponential.
+// thread). Per pair of elements that leaves five packed-fp32 instructions and two exponentials.
 // Sums: a tile's 32 shares are added in two packed chains and then join the running sum, so a sum over
 // 16384 queries is a chain of 256 additions and not of 16384.
 #include <cuda_runtime.h>
+#include <type_traits>
 
 #include "attn_common.cuh"
 #include "key_weights.h"
@@ -26,13 +26,14 @@ namespace sisa {
 namespace kwt {
 
 constexpr int BK = 128, BQ = 64, NSTAGE = 4, NCW = 8;            // keys, queries per tile, stages, compute warps
+constexpr int NG = NCW / 4, NC = BQ / NG;                        // warps per key row, query columns of each
 constexpr uint32_t SZ_K = BK * 128, SZ_B = BK * 64;
 constexpr uint32_t SZ_Q = BQ * 128, SZ_C = BQ * 64, SZ_POS = BQ * 16, SZ_LSE = BQ * 4;
 constexpr uint32_t OFFS_C = SZ_Q, OFFS_POS = OFFS_C + SZ_C, OFFS_LSE = OFFS_POS + SZ_POS;
 constexpr uint32_t SZ_STAGE = 14 * 1024;
 static_assert(OFFS_LSE + SZ_LSE <= SZ_STAGE, "stage");
 constexpr uint32_t OFF_K = 0, OFF_B = OFF_K + SZ_K, OFF_ST = OFF_B + SZ_B;
-constexpr uint32_t OFF_SUM = OFF_ST + NSTAGE * SZ_STAGE, OFF_BAR = OFF_SUM + BK * 4;
+constexpr uint32_t OFF_SUM = OFF_ST + NSTAGE * SZ_STAGE, OFF_BAR = OFF_SUM + (NG - 1) * BK * 4;
 constexpr uint32_t SMEM_BYTES = OFF_BAR + 256 + 1024;
 static_assert(OFF_ST % 1024 == 0 && SZ_STAGE % 1024 == 0, "swizzle alignment");
 static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
   if (tid == 0) {
     mbar_init(BAR(B_K), 1);
     for (int s = 0; s < NSTAGE; ++s) {
-      mbar_init(BAR(B_QF + s), 33);                // the TMA bytes and 32 lanes' lse values
+      mbar_init(BAR(B_QF + s), 33);                // the TMA bytes and 32 lanes' query terms
       mbar_init(BAR(B_QE + s), NCW + 1);           // the compute warps and the UMMAs
     }
     for (int u = 0; u < 2; ++u) {
@@ -86,8 +87,13 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
       tma_load_4d(sK, &p.tm_k, BAR(B_K), 0, k0, h, b);
       tma_load_4d(sB, &p.tm_b, BAR(B_K), 0, k0, h, b);
     }
+    // per query of the tile a_i = (F_i - F of the tile's first query) log2e - lse_i: taken relative to the
+    // tile, the difference keeps the precision that F itself, a sum over the whole prompt, would cost
     const float* lse = p.lse + (int64_t)bh * L;
-    auto lse_at = [&](int i) { return i < L ? -__ldg(lse + i) : 0.f; };
+    const float* fpl = p.pos + (int64_t)bh * 4 * p.Lp + p.Lp;
+    auto f_at = [&](int i) { return i < L ? __ldg(fpl + i) : 0.f; };
+    auto lse_at = [&](int i) { return i < L ? __ldg(lse + i) : 0.f; };
+    float f0 = f_at(i_begin + lane), f1 = f_at(i_begin + lane + 32);
     float n0 = lse_at(i_begin + lane), n1 = lse_at(i_begin + lane + 32);
     for (int n = 0; n < ntiles; ++n) {
       const int s = n % NSTAGE, i0 = i_begin + n * BQ;
@@ -100,9 +106,12 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
         tma_load_3d(st + OFFS_POS, &p.tm_pos, BAR(B_QF + s), i0, 0, bh);
       }
       float* nl = reinterpret_cast<float*>(gbase + OFF_ST + s * SZ_STAGE + OFFS_LSE);
-      nl[lane] = n0;                               // -lse of this tile's queries
-      nl[lane + 32] = n1;
+      const float fr = __shfl_sync(0xffffffffu, f0, 0);
+      nl[lane] = fmaf(f0 - fr, kLOG2E, -n0);
+      nl[lane + 32] = fmaf(f1 - fr, kLOG2E, -n1);
       mbar_arrive(BAR(B_QF + s));
+      f0 = f_at(i0 + BQ + lane);
+      f1 = f_at(i0 + BQ + lane + 32);
       n0 = lse_at(i0 + BQ + lane);                 // the next tile's, in flight while this warp waits
       n1 = lse_at(i0 + BQ + lane + 32);
     }
@@ -128,61 +137,76 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
     }
   } else {
     // ------------------------------------------------------------------ compute
-    const int r = tid & 127, half = warp >> 2;     // key row of the tile, which 32 query columns
+    const int r = tid & 127, grp = warp >> 2;      // key row of the tile, which NC query columns
     const int j = k0 + r;
     const float* posbh = p.pos + (int64_t)bh * 4 * p.Lp;
     const int jj = min(j, L - 1), je = min(k0 + BK, L) - 1;
     const float gj = posbh[jj], fj = posbh[p.Lp + jj], gend = posbh[je];
     const float lam2 = p.lam[h] * kLOG2E;
     const float cj = lam2 * exp2f(fmin_nan((gend - gj) * kLOG2E, 0.f));
-    const float2 nfj = bcast2(-fj), l2e = bcast2(kLOG2E), c1 = bcast2(kScale * kLOG2E);
+    const float2 c1 = bcast2(kScale * kLOG2E);
     float2 total = bcast2(0.f);
     bool ok = true;
     for (int n = 0; n < ntiles; ++n) {
       const int s = n % NSTAGE, u = n & 1, i0 = i_begin + n * BQ;
-      // the scores, and the lse values that the producer's lanes stored
+      // the scores, and the query terms that the producer's lanes stored
       if (!warp_wait_tested<true>(BAR(B_SF + u), (n >> 1) & 1, p.status) ||
           !warp_wait_tested<true>(BAR(B_QF + s), (n / NSTAGE) & 1, p.status)) { ok = false; break; }
       tc_fence_after();
-      float sv[32], uv[32];
-      tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + half * 32), sv);
-      tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + 64 + half * 32), uv);
+      float sv[NC], uv[NC];
+      if constexpr (NC == 32) {
+        tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + grp * NC), sv);
+        tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + 64 + grp * NC), uv);
+      } else {
+        tmem_ld16(tmem_addr(tbase, warp & 3, u * 128 + grp * NC), sv);
+        tmem_ld16(tmem_addr(tbase, warp & 3, u * 128 + 64 + grp * NC), uv);
+      }
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR(B_SE + u));   // the buffer may take the tile after next
       const float* q = reinterpret_cast<const float*>(gbase + OFF_ST + s * SZ_STAGE + OFFS_POS);
-      const float4* qf4 = reinterpret_cast<const float4*>(q + BQ) + half * 8;           // F_i
-      const float4* qr4 = reinterpret_cast<const float4*>(q + 2 * BQ) + half * 8;       // decay within the block
-      const float4* ql4 = reinterpret_cast<const float4*>(q + 4 * BQ) + half * 8;       // -lse_i
+      const float4* qr4 = reinterpret_cast<const float4*>(q + 2 * BQ) + grp * (NC / 4);       // decay within the block
+      const float4* ql4 = reinterpret_cast<const float4*>(q + 4 * BQ) + grp * (NC / 4);       // a_i
       float2 t0 = bcast2(0.f), t1 = bcast2(0.f);
-      if (i0 >= k0 + BK && i0 >= p.first && i0 + BQ <= L) {
+      const int c0 = i0 + grp * NC;                // this thread's first query
+      // off the diagonal: the decay by factors. kMask: the tile reaches before `first` or past L
+      auto factored = [&](auto mask) {
+        constexpr bool kMask = decltype(mask)::value;
+        const float2 cf = bcast2((q[BQ] - fj) * kLOG2E);
         const float2 cm = bcast2(cj * exp2f(fmin_nan((q[0] - gend) * kLOG2E, 0.f)));
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float4 f4 = qf4[c], r4 = qr4[c], l4 = ql4[c];
+        for (int c = 0; c < NC / 4; ++c) {
+          const float4 r4 = qr4[c], l4 = ql4[c];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float2 fi = e ? make_float2(f4.z, f4.w) : make_float2(f4.x, f4.y);
             const float2 rf = e ? make_float2(r4.z, r4.w) : make_float2(r4.x, r4.y);
-            const float2 nl = e ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+            const float2 a = e ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
             const int at = 4 * c + 2 * e;
-            const float2 y = fma2(add2(fi, nfj), l2e, nl);
-            const float2 d = fma2(mul2(make_float2(uv[at], uv[at + 1]), rf), cm, y);
+            const float2 d = fma2(mul2(make_float2(uv[at], uv[at + 1]), rf), cm, add2(a, cf));
             const float2 x = fma2(make_float2(sv[at], sv[at + 1]), c1, d);
-            const float2 pe = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            float2 pe = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            if constexpr (kMask) {
+              if (c0 + at < p.first || c0 + at >= L) pe.x = 0.f;
+              if (c0 + at + 1 < p.first || c0 + at + 1 >= L) pe.y = 0.f;
+            }
             if (e) t1 = add2(t1, pe); else t0 = add2(t0, pe);
           }
         }
-      } else {
-        // tiles on the diagonal, at `first` or at the end: pairwise decay, masked shares
-        const float* qg = q + half * 32;
+      };
+      if (i0 >= k0 + BK) {
+        if (i0 >= p.first && i0 + BQ <= L) factored(std::false_type{});
+        else factored(std::true_type{});
+      } else if (c0 + NC > k0 + (warp & 3) * 32) {
+        // on the diagonal: pairwise decay, shares of later queries only (a warp whose keys all come after its
+        // queries has none)
+        const float* qg = q + grp * NC;
+        const float y = (q[BQ] - fj) * kLOG2E;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const int i = i0 + half * 32 + c;
-          const float dec = exp2f(fmin_nan((qg[c] - gj) * kLOG2E, 0.f));
-          const float y = fmaf(qg[BQ + c] - fj, kLOG2E, qg[4 * BQ + c]);
-          const float x = fmaf(sv[c], kScale * kLOG2E, fmaf(uv[c] * dec, lam2, y));
+        for (int c = 0; c < NC; ++c) {
+          const int i = c0 + c;
+          const float dec = ex2_approx(fmin_nan((qg[c] - gj) * kLOG2E, 0.f));
+          const float x = fmaf(sv[c], kScale * kLOG2E, fmaf(uv[c] * dec, lam2, y + qg[4 * BQ + c]));
           const float pe = (i >= j && i >= p.first && i < L) ? ex2_approx(x) : 0.f;
           if (c & 1) t0.y += pe; else t0.x += pe;
         }
@@ -193,10 +217,12 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
     }
     float* sums = reinterpret_cast<float*>(gbase + OFF_SUM);
     const float mine = total.x + total.y;
-    if (half) sums[r] = mine;
+    if (grp) sums[(grp - 1) * BK + r] = mine;
     named_bar_sync(1, NCW * 32);
-    if (!half && j < L) {
-      const float w = mine + sums[r];
+    if (!grp && j < L) {
+      float w = mine;
+#pragma unroll
+      for (int e = 0; e < NG - 1; ++e) w += sums[e * BK + r];
       p.w[(int64_t)bh * L + j] = w;
       if (ok && !isfinite(w) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
     }
