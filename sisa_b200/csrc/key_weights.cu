@@ -9,13 +9,17 @@
 //              sum over queries is thread-local and the two halves meet once at the end,
 //   warp 8     TMA producer of the Q, C and position tiles; its lanes also form the queries' additive terms,
 //   warp 9     UMMA issuer and TMEM owner.
-// Per tile S^T = K Q^T (M128 N64 K64) and U^T = B~ C^T (K32) land in one of two TMEM buffers, so the next
-// tile's GEMMs run under this tile's arithmetic; two CTAs share an SM (2 x 256 TMEM columns).
+// Per tile S^T = K Q^T (M128 N64 K64) and U^T = B~ C^T (K32) land in tensor memory; the threads read them 16
+// columns at a time, so that 64 registers do and three CTAs share an SM, whose GEMMs, loads and arithmetic
+// overlap (two CTAs with two TMEM buffers each: the same time with all queries, 82 -> 96 us for the last 256
+// queries of 8 x 16 heads x 4096, where a CTA lives for few tiles).
 // Off the diagonal the decay is the product of three factors <= 1: the query's within its 64-row block (a
 // stored plane), the one between the blocks (one per tile) and the key's to the end of its tile (one per
 // thread). Per pair of elements that leaves five packed-fp32 instructions and two exponentials.
 // Sums: a tile's 32 shares are added in two packed chains and then join the running sum, so a sum over
 // 16384 queries is a chain of 256 additions and not of 16384.
+// Bound: the exponential unit (16 a clock and SM) would need 119 us for the 5.4e8 pairs of 4 x 16 heads x
+// 4096; 260 us measured, with the issue slots about 60 % and the exponential unit about half busy.
 #include <cuda_runtime.h>
 #include <type_traits>
 
@@ -25,8 +29,8 @@
 namespace sisa {
 namespace kwt {
 
-constexpr int BK = 128, BQ = 64, NSTAGE = 4, NCW = 8;            // keys, queries per tile, stages, compute warps
-constexpr int NG = NCW / 4, NC = BQ / NG;                        // warps per key row, query columns of each
+constexpr int BK = 128, BQ = 64, NSTAGE = 3, NCW = 8;            // keys, queries per tile, stages, compute warps
+constexpr int NG = NCW / 4, NC = BQ / NG, CH = 16;              // warps per key row, query columns of each, columns at a time
 constexpr uint32_t SZ_K = BK * 128, SZ_B = BK * 64;
 constexpr uint32_t SZ_Q = BQ * 128, SZ_C = BQ * 64, SZ_POS = BQ * 16, SZ_LSE = BQ * 4;
 constexpr uint32_t OFFS_C = SZ_Q, OFFS_POS = OFFS_C + SZ_C, OFFS_LSE = OFFS_POS + SZ_POS;
@@ -36,14 +40,14 @@ constexpr uint32_t OFF_K = 0, OFF_B = OFF_K + SZ_K, OFF_ST = OFF_B + SZ_B;
 constexpr uint32_t OFF_SUM = OFF_ST + NSTAGE * SZ_STAGE, OFF_BAR = OFF_SUM + (NG - 1) * BK * 4;
 constexpr uint32_t SMEM_BYTES = OFF_BAR + 256 + 1024;
 static_assert(OFF_ST % 1024 == 0 && SZ_STAGE % 1024 == 0, "swizzle alignment");
-static_assert(2 * (SMEM_BYTES + 1024) <= 228 * 1024, "two CTAs per SM");
-constexpr uint32_t TMEM_COLS = 256;                              // two buffers of S^T (64) and U^T (64)
-constexpr int B_K = 0, B_QF = 1, B_QE = B_QF + NSTAGE, B_SF = B_QE + NSTAGE, B_SE = B_SF + 2;
-static_assert((B_SE + 2) * 8 <= 128, "barriers end below the TMEM slot");
+static_assert(3 * (SMEM_BYTES + 1024) <= 228 * 1024, "three CTAs per SM");
+constexpr uint32_t TMEM_COLS = 128;                              // S^T (64) and U^T (64)
+constexpr int B_K = 0, B_QF = 1, B_QE = B_QF + NSTAGE, B_SF = B_QE + NSTAGE, B_SE = B_SF + 1;
+static_assert((B_SE + 1) * 8 <= 128, "barriers end below the TMEM slot");
 constexpr int NT = (NCW + 2) * 32;
 
 template <bool kHalf>
-__global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constant__ KeyWeightParams p) {
+__global__ void __launch_bounds__(NT, 3) key_weights_kernel(const __grid_constant__ KeyWeightParams p) {
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int bh, kt;
@@ -68,10 +72,8 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
       mbar_init(BAR(B_QF + s), 33);                // the TMA bytes and 32 lanes' query terms
       mbar_init(BAR(B_QE + s), NCW + 1);           // the compute warps and the UMMAs
     }
-    for (int u = 0; u < 2; ++u) {
-      mbar_init(BAR(B_SF + u), 1);
-      mbar_init(BAR(B_SE + u), NCW);
-    }
+    mbar_init(BAR(B_SF), 1);
+    mbar_init(BAR(B_SE), NCW);
     fence_barrier_init();
   }
   if (warp == NCW + 1) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
@@ -121,17 +123,17 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
       constexpr uint32_t idesc = make_idesc(128, 64, kHalf ? 0 : 1, 0, 0);
       bool ok = mbar_wait<true>(BAR(B_K), 0, p.status);
       for (int n = 0; ok && n < ntiles; ++n) {
-        const int s = n % NSTAGE, u = n & 1;
+        const int s = n % NSTAGE;
         if (!mbar_wait<true>(BAR(B_QF + s), (n / NSTAGE) & 1, p.status)) break;
-        if (n >= 2 && !mbar_wait<true>(BAR(B_SE + u), ((n >> 1) - 1) & 1, p.status)) break;
+        if (n >= 1 && !mbar_wait<true>(BAR(B_SE), (n - 1) & 1, p.status)) break;
         tc_fence_after();
-        const uint32_t st = stage_addr(s), tS = tbase + u * 128, tU = tS + 64;
+        const uint32_t st = stage_addr(s), tS = tbase, tU = tbase + 64;
 #pragma unroll
         for (int k = 0; k < 4; ++k) umma_ss(tS, desc_k128(sK + k * 32), desc_k128(st + k * 32), idesc, k > 0);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
           umma_ss(tU, desc_k64(sB + k * 32), desc_k64(st + OFFS_C + k * 32), idesc, k > 0);
-        umma_commit(BAR(B_SF + u));
+        umma_commit(BAR(B_SF));
         umma_commit(BAR(B_QE + s));
       }
     }
@@ -148,67 +150,67 @@ __global__ void __launch_bounds__(NT, 2) key_weights_kernel(const __grid_constan
     float2 total = bcast2(0.f);
     bool ok = true;
     for (int n = 0; n < ntiles; ++n) {
-      const int s = n % NSTAGE, u = n & 1, i0 = i_begin + n * BQ;
+      const int s = n % NSTAGE, i0 = i_begin + n * BQ;
       // the scores, and the query terms that the producer's lanes stored
-      if (!warp_wait_tested<true>(BAR(B_SF + u), (n >> 1) & 1, p.status) ||
+      if (!warp_wait_tested<true>(BAR(B_SF), n & 1, p.status) ||
           !warp_wait_tested<true>(BAR(B_QF + s), (n / NSTAGE) & 1, p.status)) { ok = false; break; }
       tc_fence_after();
-      float sv[NC], uv[NC];
-      if constexpr (NC == 32) {
-        tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + grp * NC), sv);
-        tmem_ld32(tmem_addr(tbase, warp & 3, u * 128 + 64 + grp * NC), uv);
-      } else {
-        tmem_ld16(tmem_addr(tbase, warp & 3, u * 128 + grp * NC), sv);
-        tmem_ld16(tmem_addr(tbase, warp & 3, u * 128 + 64 + grp * NC), uv);
-      }
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(BAR(B_SE + u));   // the buffer may take the tile after next
       const float* q = reinterpret_cast<const float*>(gbase + OFF_ST + s * SZ_STAGE + OFFS_POS);
       const float4* qr4 = reinterpret_cast<const float4*>(q + 2 * BQ) + grp * (NC / 4);       // decay within the block
       const float4* ql4 = reinterpret_cast<const float4*>(q + 4 * BQ) + grp * (NC / 4);       // a_i
+      const bool off = i0 >= k0 + BK;              // off the diagonal
+      const float2 cf = bcast2((q[BQ] - fj) * kLOG2E);
       float2 t0 = bcast2(0.f), t1 = bcast2(0.f);
-      const int c0 = i0 + grp * NC;                // this thread's first query
-      // off the diagonal: the decay by factors. kMask: the tile reaches before `first` or past L
-      auto factored = [&](auto mask) {
-        constexpr bool kMask = decltype(mask)::value;
-        const float2 cf = bcast2((q[BQ] - fj) * kLOG2E);
-        const float2 cm = bcast2(cj * exp2f(fmin_nan((q[0] - gend) * kLOG2E, 0.f)));
 #pragma unroll
-        for (int c = 0; c < NC / 4; ++c) {
-          const float4 r4 = qr4[c], l4 = ql4[c];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 rf = e ? make_float2(r4.z, r4.w) : make_float2(r4.x, r4.y);
-            const float2 a = e ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
-            const int at = 4 * c + 2 * e;
-            const float2 d = fma2(mul2(make_float2(uv[at], uv[at + 1]), rf), cm, add2(a, cf));
-            const float2 x = fma2(make_float2(sv[at], sv[at + 1]), c1, d);
-            float2 pe = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            if constexpr (kMask) {
-              if (c0 + at < p.first || c0 + at >= L) pe.x = 0.f;
-              if (c0 + at + 1 < p.first || c0 + at + 1 >= L) pe.y = 0.f;
-            }
-            if (e) t1 = add2(t1, pe); else t0 = add2(t0, pe);
-          }
+      for (int ch = 0; ch < NC; ch += CH) {
+        float sv[CH], uv[CH];
+        tmem_ld16(tmem_addr(tbase, warp & 3, grp * NC + ch), sv);
+        tmem_ld16(tmem_addr(tbase, warp & 3, 64 + grp * NC + ch), uv);
+        tmem_wait_ld();
+        if (ch + CH == NC) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(BAR(B_SE));
         }
-      };
-      if (i0 >= k0 + BK) {
-        if (i0 >= p.first && i0 + BQ <= L) factored(std::false_type{});
-        else factored(std::true_type{});
-      } else if (c0 + NC > k0 + (warp & 3) * 32) {
-        // on the diagonal: pairwise decay, shares of later queries only (a warp whose keys all come after its
-        // queries has none)
-        const float* qg = q + grp * NC;
-        const float y = (q[BQ] - fj) * kLOG2E;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int i = c0 + c;
-          const float dec = ex2_approx(fmin_nan((qg[c] - gj) * kLOG2E, 0.f));
-          const float x = fmaf(sv[c], kScale * kLOG2E, fmaf(uv[c] * dec, lam2, y + qg[4 * BQ + c]));
-          const float pe = (i >= j && i >= p.first && i < L) ? ex2_approx(x) : 0.f;
-          if (c & 1) t0.y += pe; else t0.x += pe;
+        const int c0 = i0 + grp * NC + ch;         // this thread's first query
+        // the decay by factors. kMask: the tile reaches before `first` or past L
+        auto factored = [&](auto mask) {
+          constexpr bool kMask = decltype(mask)::value;
+          const float2 cm = bcast2(cj * exp2f(fmin_nan((q[0] - gend) * kLOG2E, 0.f)));
+  #pragma unroll
+          for (int c = 0; c < CH / 4; ++c) {
+            const float4 r4 = qr4[c + ch / 4], l4 = ql4[c + ch / 4];
+  #pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 rf = e ? make_float2(r4.z, r4.w) : make_float2(r4.x, r4.y);
+              const float2 a = e ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+              const int at = 4 * c + 2 * e;
+              const float2 d = fma2(mul2(make_float2(uv[at], uv[at + 1]), rf), cm, add2(a, cf));
+              const float2 x = fma2(make_float2(sv[at], sv[at + 1]), c1, d);
+              float2 pe = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              if constexpr (kMask) {
+                if (c0 + at < p.first || c0 + at >= L) pe.x = 0.f;
+                if (c0 + at + 1 < p.first || c0 + at + 1 >= L) pe.y = 0.f;
+              }
+              if (e) t1 = add2(t1, pe); else t0 = add2(t0, pe);
+            }
+          }
+        };
+        if (off) {
+          if (i0 >= p.first && i0 + BQ <= L) factored(std::false_type{});
+          else factored(std::true_type{});
+        } else if (c0 + CH > k0 + (warp & 3) * 32) {
+          // on the diagonal: pairwise decay, shares of later queries only (a warp whose keys all come after its
+          // queries has none)
+          const float* qg = q + grp * NC + ch;
+  #pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            const int i = c0 + c;
+            const float dec = ex2_approx(fmin_nan((qg[c] - gj) * kLOG2E, 0.f));
+            const float x = fmaf(sv[c], kScale * kLOG2E, fmaf(uv[c] * dec, lam2, cf.x + qg[4 * BQ + c]));
+            const float pe = (i >= j && i >= p.first && i < L) ? ex2_approx(x) : 0.f;
+            if (c & 1) t0.y += pe; else t0.x += pe;
+          }
         }
       }
       __syncwarp();
