@@ -219,6 +219,7 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
   __shared__ int s_hist[BINS], s_warp[32], s_base[ST], s_tie[ST];
   __shared__ uint32_t s_digit;
   __shared__ int s_left;
+  __shared__ bool s_whole;
   asm volatile("griddepcontrol.launch_dependents;");
   const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int32_t* out = p.index + (int64_t)bh * p.keep;
@@ -254,14 +255,24 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
       const int d = BINS - 1 - 2 * tid, h0 = s_hist[d], h1 = s_hist[d - 1];
       int total;
       const int over = scan_excl(h0 + h1, s_warp, total);
-      if (over < left && left <= over + h0) { s_digit = d; s_left = left - over; }
-      else if (over + h0 < left && left <= over + h0 + h1) { s_digit = d - 1; s_left = left - over - h0; }
+      if (over < left && left <= over + h0) { s_digit = d; s_left = left - over; s_whole = left == over + h0; }
+      else if (over + h0 < left && left <= over + h0 + h1) {
+        s_digit = d - 1;
+        s_left = left - over - h0;
+        s_whole = left == over + h0 + h1;
+      }
       __syncthreads();
       prefix |= s_digit << shift;
       left = s_left;
-      __syncthreads();
+      if (s_whole && prefix > 0) {               // the whole digit is kept: no need to look further into it
+        --prefix;
+        left = 0;
+        break;
+      }
+      // (the next pass's first barrier keeps these until every thread has read them)
     }
   }
+  __syncthreads();
   // with left == 0 nothing but the newest is kept: no key is above the largest order
   if (p.keep == p.recent) prefix = 0xffffffffu;
   int done = 0, ties = 0;                        // kept, and keys at T, in the chunks before
@@ -305,52 +316,46 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
   }
 }
 
-// 64 kept keys of one unit per block: eight lanes per key copy its rows (16 bytes a lane, two keys a lane so
-// that six loads are in flight), 64 threads its plane values, into the sequence's pages.
-constexpr int GK = 64;
+// 32 kept keys of one unit per block: eight lanes per key copy its rows (16 bytes a lane), 32 threads its
+// plane values, into the sequence's pages. The units are the fast grid dimension, so the blocks in flight
+// read the same part of the prompt for all heads, whose rows lie side by side in the projection. (Two keys
+// a lane: 101 instead of 97 us for 16 x 16 units of 8192 -> 2048 keys, four: 122 us.)
+constexpr int GK = 32;
 __global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
-  const int bh = blockIdx.y, b = bh / p.H, h = bh % p.H, tid = threadIdx.x;
-  const int64_t r0 = (int64_t)blockIdx.x * GK;
-  const int part = tid & 7;
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, tid = threadIdx.x, part = tid & 7;
   const int32_t* index = p.index + (int64_t)bh * p.keep;
-  int pages[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t r = r0 + i * 32 + (tid >> 3);
-    pages[i] = r < p.keep ? page_of(p.pg, b, r, p.status) : -1;
-  }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  uint4 k[2], v[2], m[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t r = r0 + i * 32 + (tid >> 3);
-    if (pages[i] < 0) continue;
-    const int64_t j = index[r];
-    k[i] = __ldg(reinterpret_cast<const uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + j * p.k_sl)) + part);
-    v[i] = __ldg(reinterpret_cast<const uint4*>(p.v + 2 * (b * p.v_sb + h * p.v_sh + j * p.v_sl)) + part);
-    if (part < 4) m[i] = __ldg(reinterpret_cast<const uint4*>(p.b + 2 * (b * p.b_sb + h * p.b_sh + j * p.b_sl)) + part);
-  }
-  if (tid < GK && r0 + tid < p.keep) {
-    const int64_t r = r0 + tid, j = index[r];
-    const int page = page_of(p.pg, b, r, nullptr);
-    if (page >= 0) {
-      const int64_t at = page * p.pg.s_sp + h * p.pg.s_sh + (r & ((1 << p.pg.page_shift) - 1));
-      const float g = __ldg(p.g + b * p.g_sb + h * p.g_sh + j);
-      const float f = p.f ? __ldg(p.f + b * p.f_sb + h * p.f_sh + j) : 0.f;
-      const float w = p.weight ? __ldg(p.weight + (int64_t)bh * p.L + j) : 0.f;
-      p.pg.g[at] = g;
-      if (p.pg.f) p.pg.f[at] = f;
-      if (p.pg.weight) p.pg.weight[at] = w;
-      if (p.pg.token) p.pg.token[at] = (int)j;
+  bool waited = false;
+  for (int64_t r0 = (int64_t)blockIdx.y * GK; r0 < p.keep; r0 += (int64_t)gridDim.y * GK) {
+    const int64_t r = r0 + (tid >> 3);
+    const int page = r < p.keep ? page_of(p.pg, b, r, p.status) : -1;
+    if (!waited) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      waited = true;
     }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t in = (r0 + i * 32 + (tid >> 3)) & ((1 << p.pg.page_shift) - 1), page = pages[i];
-    if (page < 0) continue;
-    reinterpret_cast<uint4*>(p.pg.k + 2 * (page * p.pg.k_sp + h * p.pg.k_sh + in * 64))[part] = k[i];
-    reinterpret_cast<uint4*>(p.pg.v + 2 * (page * p.pg.v_sp + h * p.pg.v_sh + in * 64))[part] = v[i];
-    if (part < 4) reinterpret_cast<uint4*>(p.pg.b + 2 * (page * p.pg.b_sp + h * p.pg.b_sh + in * 32))[part] = m[i];
+    if (page >= 0) {
+      const int64_t j = index[r], in = r & ((1 << p.pg.page_shift) - 1);
+      const uint4 k = __ldg(reinterpret_cast<const uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + j * p.k_sl)) + part);
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.v + 2 * (b * p.v_sb + h * p.v_sh + j * p.v_sl)) + part);
+      uint4 m = make_uint4(0, 0, 0, 0);
+      if (part < 4) m = __ldg(reinterpret_cast<const uint4*>(p.b + 2 * (b * p.b_sb + h * p.b_sh + j * p.b_sl)) + part);
+      reinterpret_cast<uint4*>(p.pg.k + 2 * (page * p.pg.k_sp + h * p.pg.k_sh + in * 64))[part] = k;
+      reinterpret_cast<uint4*>(p.pg.v + 2 * (page * p.pg.v_sp + h * p.pg.v_sh + in * 64))[part] = v;
+      if (part < 4) reinterpret_cast<uint4*>(p.pg.b + 2 * (page * p.pg.b_sp + h * p.pg.b_sh + in * 32))[part] = m;
+    }
+    if (tid < GK && r0 + tid < p.keep) {
+      const int64_t rr = r0 + tid, j = index[rr];
+      const int pp = page_of(p.pg, b, rr, nullptr);
+      if (pp >= 0) {
+        const int64_t at = pp * p.pg.s_sp + h * p.pg.s_sh + (rr & ((1 << p.pg.page_shift) - 1));
+        const float g = __ldg(p.g + b * p.g_sb + h * p.g_sh + j);
+        const float f = p.f ? __ldg(p.f + b * p.f_sb + h * p.f_sh + j) : 0.f;
+        const float w = p.weight ? __ldg(p.weight + (int64_t)bh * p.L + j) : 0.f;
+        p.pg.g[at] = g;
+        if (p.pg.f) p.pg.f[at] = f;
+        if (p.pg.weight) p.pg.weight[at] = w;
+        if (p.pg.token) p.pg.token[at] = (int)j;
+      }
+    }
   }
 }
 
@@ -390,7 +395,8 @@ cudaError_t launch_paged_fill(const PagedFillParams& p, cudaStream_t st) {
   pca::paged_select_kernel<<<p.B * p.H, pca::ST, smem, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((p.keep + pca::GK - 1) / pca::GK), p.B * p.H);
+  const int64_t chunks = (p.keep + pca::GK - 1) / pca::GK;
+  cfg.gridDim = dim3(p.B * p.H, (unsigned)(chunks < 65535 ? chunks : 65535));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
