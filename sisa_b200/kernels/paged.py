@@ -67,7 +67,6 @@ class KeyPages:
                              _lib.ptr(token), k.stride(0), k.stride(1), v.stride(0), v.stride(1), b.stride(0), b.stride(1),
                              g.stride(0), g.stride(1), P, S)
         self.cbytes = bytes(c)                  # the struct every call passes
-        self.dev_index = k.device.index if k.device.index is not None else 0
 
     @classmethod
     def empty(cls, n_pages: int, n_head: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda",
@@ -168,9 +167,9 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
         c = c.to(q.dtype)
     q, c, gq, lam = _operand(q), _operand(c), _f32(g), _f32(lam)
     fq = None if fgate is None else _f32(fgate)
-    y = torch.empty((B, H, 1, 64), device=dev, dtype=q.dtype)
-    lse = torch.empty((B, H), device=dev, dtype=torch.float32) if return_lse else None
-    ws = torch.empty(lib.sisa_paged_attn_workspace(B, H, mp * pages.page_size, accumulate), dtype=torch.uint8, device=dev)
+    y = q.new_empty((B, H, 1, 64))              # (new_empty costs less host time than torch.empty with a device)
+    lse = lam.new_empty((B, H)) if return_lse else None
+    ws = lam.new_empty(lib.sisa_paged_attn_workspace(B, H, mp * pages.page_size, accumulate) // 4)
     rc = lib.sisa_paged_attn(_lib.view4_bytes(q), _lib.view4_bytes(c), gq.data_ptr(), None if fq is None else fq.data_ptr(),
                              pages.cbytes, tp, tsb, mp, lp, lam.data_ptr(), B, H, pages.dtype_code, _lib.view4_bytes(y),
                              None if lse is None else lse.data_ptr(), None if wo is None else wo.data_ptr(), ws.data_ptr(),
@@ -188,7 +187,7 @@ def paged_evict(pages: KeyPages, block_table: Tensor, position: Tensor, budget: 
     tp, tsb, mp = _table(pages, block_table, B)
     pp = _rows(position, (B,), "position", pages)
     dev = pages.device
-    slots = torch.empty((B, H), dtype=torch.int32, device=dev)
+    slots = position.new_empty((B, H))
     rc = _lib.load().sisa_paged_evict(pages.cbytes, tp, tsb, mp, pp, B, H, int(budget), int(recent), slots.data_ptr(),
                                       backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_evict")
@@ -233,8 +232,8 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
             wide = proj.new_empty((B, 1, -(-width // 8) * 8))
             wide[..., :width] = proj
             proj, sb = wide, wide.shape[2]
-    c = torch.empty((B, H, 1, 32), dtype=proj.dtype, device=dev)
-    g = torch.empty((B, H, 1), dtype=torch.float32, device=dev)
+    c = proj.new_empty((B, H, 1, 32))
+    g = carry.new_empty((B, H, 1))
     z2 = f = zp = fp = None
     if z is not None:
         if pages.f is None:
@@ -242,7 +241,7 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
         if z.numel() != B * H or z.device != dev:
             raise ValueError(f"z must be ({B}, 1, {H}) on {dev}, got {tuple(z.shape)} on {z.device}")
         z2 = _f32(z)
-        f = torch.empty((B, H, 1), dtype=torch.float32, device=dev)
+        f = carry.new_empty((B, H, 1))
         zp, fp = z2.data_ptr(), f.data_ptr()
     rc = _lib.load().sisa_paged_append(proj.data_ptr(), sb if B > 1 else width, zp, H, pages.cbytes, tp, tsb, mp, pp, sp,
                                        int(budget or 0), B, H, pages.dtype_code, carry.data_ptr(), co.data_ptr(),
@@ -281,7 +280,7 @@ def attention_key_weights(q: Tensor, k: Tensor, c: Tensor, b: Tensor, pos: Tenso
     if any(t.device != dev for t in (k, c, b, pos, lam, lse)) or not q.is_cuda:
         raise ValueError("attention_key_weights takes CUDA tensors on one device")
     q, k, c, b, lse = _operand(q), _operand(k), _operand(c), _operand(b), lse.contiguous()
-    w = torch.empty((B, H, L), dtype=torch.float32, device=dev)
+    w = lse.new_empty((B, H, L))
     rc = lib.sisa_attn_key_weights(*map(_lib.view4_bytes, (q, k, c, b)), pos.data_ptr(), lam.data_ptr(), lse.data_ptr(), B,
                                    H, L, int(first_query), code, w.data_ptr(), backends.status_word(dev).data_ptr(),
                                    _lib.stream_ptr(dev))
@@ -299,28 +298,29 @@ def paged_fill(pages: KeyPages, block_table: Tensor, k: Tensor, v: Tensor, b: Te
     if k.dim() != 4 or k.shape[-1] != 64:
         raise ValueError(f"k must be (B, H, L, 64), got {tuple(k.shape)}")
     B, H, L, _ = k.shape
-    if H != pages.n_head or tuple(v.shape) != (B, H, L, 64) or tuple(b.shape) != (B, H, L, 32):
+    if H != pages.n_head or v.shape != (B, H, L, 64) or b.shape != (B, H, L, 32):
         raise ValueError(f"k, v and b must be (B, {pages.n_head}, L, 64), (.., 64) and (.., 32), got {tuple(k.shape)}, "
                          f"{tuple(v.shape)} and {tuple(b.shape)}")
-    if any(t.dtype != pages.dtype for t in (k, v, b)):
+    if k.dtype != pages.dtype or v.dtype != pages.dtype or b.dtype != pages.dtype:
         raise TypeError(f"k, v and b must be {pages.dtype} like the pages, got {k.dtype}, {v.dtype}, {b.dtype}")
     dev = pages.device
-    if any(t is not None and t.device != dev for t in (k, v, b, g, fgate, weight)):
-        raise ValueError(f"the prompt's keys must lie on {dev} like the pages")
+    for t in (k, v, b, g, fgate, weight):
+        if t is not None and t.device != dev:
+            raise ValueError(f"the prompt's keys must lie on {dev} like the pages")
     keep = L if keep is None else int(keep)
     if weight is not None:
-        if tuple(weight.shape) != (B, H, L) or weight.dtype != torch.float32:
+        if weight.shape != (B, H, L) or weight.dtype != torch.float32:
             raise ValueError(f"weight must be {(B, H, L)} fp32, got {tuple(weight.shape)} {weight.dtype}")
         weight = weight.contiguous()
     for name, t in (("g", g), ("fgate", fgate)):
-        if t is not None and (tuple(t.shape) != (B, H, L) or t.dtype != torch.float32):
+        if t is not None and (t.shape != (B, H, L) or t.dtype != torch.float32):
             raise ValueError(f"{name} must be {(B, H, L)} fp32, got {tuple(t.shape)} {t.dtype}")
     if fgate is not None and pages.f is None:
         raise ValueError("fgate is given but the pages hold no f plane")
     g, fgate = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (g, fgate))
     tp, tsb, mp = _table(pages, block_table, B)
     lib = _lib.load()
-    ws = torch.empty(max(lib.sisa_paged_fill_workspace(B, H, keep), 16), dtype=torch.uint8, device=dev)
+    ws = block_table.new_empty(max(B * H * min(keep, L), 4))             # the kept positions
     k, v, b = _operand(k), _operand(v), _operand(b)
     fs = (0, 0) if fgate is None else fgate.stride()[:2]
     rc = lib.sisa_paged_fill(pages.cbytes, tp, tsb, mp, *map(_lib.view4_bytes, (k, v, b)), g.data_ptr(), g.stride(0),
