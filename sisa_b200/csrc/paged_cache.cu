@@ -181,12 +181,13 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) 
 // The kept keys of one (batch, head), ascending: the last `recent`, and of the rest the keep - recent of
 // the largest weight, the earlier position where two weigh the same. One block per unit:
 //   1. a radix select over the ordered weights (11 + 11 + 10 bits) finds the smallest kept weight T and how
-//      many of the keys at T are kept;
+//      many of the keys at T are kept; it ends where a digit is kept whole, and after the first digit reads
+//      only the keys that share it;
 //   2. per 32-key group the kept keys above T and the ties are counted, two block scans (ties first: how
 //      many of them a group keeps depends on those before it) place the groups, and the kept positions
 //      are written in order.
 // The weights of up to SEL_SMEM keys are ordered once into shared memory; longer prompts are read again
-// from L2 in each pass. With it and 1024 threads a unit of 8192 keys takes about 10 us.
+// from L2 in each pass.
 constexpr int ST = 1024, SEL_SMEM = 40960;
 constexpr int BINS = 2048;
 
@@ -216,16 +217,17 @@ __device__ __forceinline__ int scan_excl(int v, int* s_warp, int& total) {
 
 __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
   extern __shared__ uint32_t s_key[];            // ordered weights of positions [0, old) when they fit
-  __shared__ int s_hist[BINS], s_warp[32], s_base[ST], s_tie[ST];
+  __shared__ int s_hist[BINS], s_warp[32];
+  // the candidates of the later passes; then per 32-key group: keys surely kept, ties, first place, ties before
+  __shared__ uint32_t s_buf[4 * ST];
   __shared__ uint32_t s_digit;
-  __shared__ int s_left;
-  __shared__ bool s_whole;
+  __shared__ int s_left, s_in, s_count;
   asm volatile("griddepcontrol.launch_dependents;");
   const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t below = (1u << lane) - 1;
   int32_t* out = p.index + (int64_t)bh * p.keep;
   const int L = (int)p.L, old = (int)(p.L - p.recent);   // positions [0, old) compete for keep - recent places
-  const bool all = p.keep == p.L;
-  if (all) {
+  if (p.keep == p.L) {
     for (int j = tid; j < L; j += ST) out[j] = j;
     return;
   }
@@ -234,10 +236,12 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
   if (in_smem) {
     for (int j = tid; j < old; j += ST) s_key[j] = weight_order(__ldg(wt + j));
   }
-  __syncthreads();
   auto key_at = [&](int j) { return in_smem ? s_key[j] : weight_order(__ldg(wt + j)); };
-  uint32_t prefix = 0;
+  // with no place left nothing but the newest is kept: no key is above the largest order
+  uint32_t prefix = p.keep == p.recent ? 0xffffffffu : 0u;
   int left = (int)(p.keep - p.recent);           // places left among the keys that match the prefix
+  int cand = -1;                                 // candidates in s_buf, -1: every key is looked at
+  if (tid == 0) s_count = 0;
   if (left > 0) {
     int shift = 32;
 #pragma unroll 1
@@ -246,69 +250,86 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
       shift -= bits;
       for (int i = tid; i < BINS; i += ST) s_hist[i] = 0;
       __syncthreads();
-      for (int j = tid; j < old; j += ST) {
-        const uint32_t u = key_at(j);
-        if (above == 32 || (u >> above) == (prefix >> above)) atomicAdd(&s_hist[(u >> shift) & ((1u << bits) - 1)], 1);
+      const uint32_t digits = (1u << bits) - 1;
+      if (cand >= 0) {
+        for (int j = tid; j < cand; j += ST) {
+          const uint32_t u = s_buf[j];
+          if ((u >> above) == (prefix >> above)) atomicAdd(&s_hist[(u >> shift) & digits], 1);
+        }
+      } else {
+        for (int j = tid; j < old; j += ST) {
+          const uint32_t u = key_at(j);
+          if (above == 32 || (u >> above) == (prefix >> above)) atomicAdd(&s_hist[(u >> shift) & digits], 1);
+        }
       }
       __syncthreads();
       // thread t holds the bins 2047 - 2t and 2046 - 2t: the scan runs from the largest digit down
       const int d = BINS - 1 - 2 * tid, h0 = s_hist[d], h1 = s_hist[d - 1];
       int total;
       const int over = scan_excl(h0 + h1, s_warp, total);
-      if (over < left && left <= over + h0) { s_digit = d; s_left = left - over; s_whole = left == over + h0; }
-      else if (over + h0 < left && left <= over + h0 + h1) {
+      if (over < left && left <= over + h0) {
+        s_digit = d;
+        s_left = left - over;
+        s_in = h0;
+      } else if (over + h0 < left && left <= over + h0 + h1) {
         s_digit = d - 1;
         s_left = left - over - h0;
-        s_whole = left == over + h0 + h1;
+        s_in = h1;
       }
       __syncthreads();
       prefix |= s_digit << shift;
       left = s_left;
-      if (s_whole && prefix > 0) {               // the whole digit is kept: no need to look further into it
+      const int in = s_in;                       // keys with this digit
+      if (left == in && prefix > 0) {            // all of them are kept: no need to look further into the digit
         --prefix;
         left = 0;
         break;
       }
-      // (the next pass's first barrier keeps these until every thread has read them)
+      if (pass == 0 && in <= 4 * ST) {           // few are left to tell apart: the later passes read only them
+        for (int j0 = 0; j0 < old; j0 += ST) {
+          const int j = j0 + tid;
+          const uint32_t u = j < old ? key_at(j) : 0u;
+          const bool is = j < old && (u >> shift) == (prefix >> shift);
+          const uint32_t m = __ballot_sync(0xffffffffu, is);
+          int at = 0;
+          if (lane == 0 && m) at = atomicAdd(&s_count, __popc(m));
+          at = __shfl_sync(0xffffffffu, at, 0);
+          if (is) s_buf[at + __popc(m & below)] = u;
+        }
+        cand = in;
+      }
+      // (the next pass's first barrier keeps the shared words until every thread has read them)
     }
   }
   __syncthreads();
-  // with left == 0 nothing but the newest is kept: no key is above the largest order
-  if (p.keep == p.recent) prefix = 0xffffffffu;
+  uint32_t* s_sure = s_buf;
+  uint32_t* s_tie = s_buf + ST;
+  int* s_base = reinterpret_cast<int*>(s_buf + 2 * ST);
+  int* s_before = reinterpret_cast<int*>(s_buf + 3 * ST);
   int done = 0, ties = 0;                        // kept, and keys at T, in the chunks before
   for (int j0 = 0; j0 < L; j0 += ST * 32) {
-    // group (warp + 32 i) of the chunk holds 32 consecutive positions
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i) {
-      const int g = warp + 32 * i, j = j0 + g * 32 + lane;
-      if (j0 + g * 32 >= L) {
-        if (lane == 0) { s_base[g] = 0; s_tie[g] = 0; }
-        continue;
-      }
+    // group g of the chunk holds 32 consecutive positions, a warp every 32nd group
+    const int groups = min(ST, (L - j0 + 31) / 32);
+    for (int g = warp; g < groups; g += 32) {
+      const int j = j0 + g * 32 + lane;
       const uint32_t u = j < old ? key_at(j) : 0u;
       const uint32_t sure = __ballot_sync(0xffffffffu, j < L && (j >= old || u > prefix));
       const uint32_t tie = __ballot_sync(0xffffffffu, j < old && u == prefix);
-      if (lane == 0) { s_base[g] = __popc(sure); s_tie[g] = __popc(tie); }
+      if (lane == 0) { s_sure[g] = sure; s_tie[g] = tie; }
     }
     __syncthreads();
     int tot_tie, tot;
-    const int nt = s_tie[tid], ns = s_base[tid];
+    const int nt = tid < groups ? __popc(s_tie[tid]) : 0, ns = tid < groups ? __popc(s_sure[tid]) : 0;
     const int tb = ties + scan_excl(nt, s_warp, tot_tie);
-    const int mine = ns + max(0, min(nt, left - tb));
-    const int at = done + scan_excl(mine, s_warp, tot);
+    const int at = done + scan_excl(ns + max(0, min(nt, left - tb)), s_warp, tot);
     s_base[tid] = at;
-    s_tie[tid] = tb;
+    s_before[tid] = tb;
     __syncthreads();
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i) {
-      const int g = warp + 32 * i, j = j0 + g * 32 + lane;
-      if (j0 + g * 32 >= L) break;
-      const uint32_t u = j < old ? key_at(j) : 0u;
-      const bool tie = j < old && u == prefix;
-      const uint32_t below = (1u << lane) - 1, ties_in = __ballot_sync(0xffffffffu, tie);
-      const bool keep = j < L && (j >= old || u > prefix || (tie && s_tie[g] + __popc(ties_in & below) < left));
-      const uint32_t kept = __ballot_sync(0xffffffffu, keep);
-      if (keep) out[s_base[g] + __popc(kept & below)] = j;
+    for (int g = warp; g < groups; g += 32) {
+      const uint32_t sure = s_sure[g], tie = s_tie[g];
+      const bool keep = ((sure >> lane) & 1) || (((tie >> lane) & 1) && s_before[g] + __popc(tie & below) < left);
+      const uint32_t kept = tie ? __ballot_sync(0xffffffffu, keep) : sure;
+      if (keep) out[s_base[g] + __popc(kept & below)] = j0 + g * 32 + lane;
     }
     __syncthreads();
     done += tot;
