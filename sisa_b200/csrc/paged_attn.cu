@@ -31,6 +31,7 @@ constexpr int TK = 32;                          // keys per tile
 constexpr int NW = 5, NSTAGE = 2;               // warps per CTA, ring stages per warp; two CTAs per SM
 constexpr int NCTA = 148 * 16;                  // eight waves: SMs stream at different rates, and the ones
                                                 // that are done take the next CTA
+constexpr int UNIT_KEYS = 512;                  // tables up to this many keys: one CTA per unit (see launch)
 constexpr int NWORK = NCTA * NW, WMIN = 296 * NW, GRAIN = 16;
 constexpr uint32_t OFF_V = TK * 128, OFF_B = OFF_V + TK * 128, OFF_G = OFF_B + TK * 64, OFF_F = OFF_G + TK * 4;
 constexpr int REC = 68;                         // floats of a record: m, l, 2 unused, acc[64]
@@ -38,7 +39,7 @@ constexpr uint32_t SZ_STAGE = OFF_F + TK * 4;   // 10,496 bytes
 constexpr uint32_t SZ_WARP = NSTAGE * SZ_STAGE;
 constexpr uint32_t OFF_REC = NW * SZ_WARP, OFF_BAR = OFF_REC + NW * 2 * REC * 4, OFF_MASK = OFF_BAR + NW * NSTAGE * 8;
 constexpr uint32_t SMEM_BYTES = OFF_MASK + NW * NSTAGE * 4 + 128;
-static_assert(SZ_STAGE % 128 == 0 && 2 * (SMEM_BYTES + 1024) <= 228 * 1024, "shared memory");
+static_assert(SZ_STAGE % 128 == 0 && 2 * (SMEM_BYTES + UNIT_KEYS * 4 + 256 + 1024) <= 228 * 1024, "shared memory");
 
 __device__ __forceinline__ int64_t keys_of(const PagedAttnParams& p, int b) {
   const int64_t n = __ldg(p.lengths + b);
@@ -171,7 +172,7 @@ struct Sum {
 
 // y and lse of unit bh = (b, h) from its complete sum.
 template <bool kHalf>
-__device__ __forceinline__ void write_row(const PagedAttnParams& p, int64_t bh, const Sum& s) {
+__device__ __forceinline__ float write_row(const PagedAttnParams& p, int64_t bh, const Sum& s) {
   const int64_t b = bh / p.H, h = bh % p.H;
   const int lane = threadIdx.x & 31;
   const float lse = s.m + log2f(s.l), r = 1.f / s.l;
@@ -180,12 +181,15 @@ __device__ __forceinline__ void write_row(const PagedAttnParams& p, int64_t bh, 
     p.lse_all[bh] = lse;
     if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
   }
+  return lse;
 }
 
-template <bool kHalf, bool kScores>
+// kUnit: a CTA has one unit to itself, its warps equal runs of that unit's tiles; y, lse and (from the scores
+// kept in shared memory) the weights are finished here and no other kernel follows.
+template <bool kHalf, bool kScores, bool kUnit>
 __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  asm volatile("griddepcontrol.launch_dependents;");
+  if constexpr (!kUnit) asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t raw = smem_u32(smem_raw), sbase = (raw + 127u) & ~127u;
   uint8_t* gbase = smem_raw + (sbase - raw);
@@ -198,23 +202,43 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
   }
   __syncwarp();
 
-  int64_t per_head;
-  tiles_before(p, 0, per_head);
-  const int64_t tiles = per_head * p.H, nwork = workers(tiles);
-  if ((int64_t)blockIdx.x * NW >= nwork && blockIdx.x > 0) return;
-  const int w = blockIdx.x * NW + warp;
-  if (w == 0) {                                 // lengths past the table, once per sequence
-    for (int b = lane; b < p.B; b += 32)
-      if (__ldg(p.lengths + b) > p.max_keys && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
+  // ---- this warp's run of tiles: count of them from cursor `in` on
+  Cursor in{}, at;
+  int64_t count = 0;
+  if constexpr (kUnit) {
+    in.b = blockIdx.x / p.H;
+    in.h = blockIdx.x % p.H;
+    in.load(p);
+    in.t = in.T * warp / NW;
+    count = in.T * (warp + 1) / NW - in.t;
+    if (in.h == 0 && threadIdx.x == 0 && __ldg(p.lengths + in.b) > p.max_keys && p.status)
+      atomicOr(p.status, SISA_ST_BAD_POS);
+  } else {
+    int64_t per_head;
+    tiles_before(p, 0, per_head);
+    const int64_t tiles = per_head * p.H, nwork = workers(tiles);
+    if ((int64_t)blockIdx.x * NW >= nwork && blockIdx.x > 0) return;
+    const int w = blockIdx.x * NW + warp;
+    if (w == 0) {                               // lengths past the table, once per sequence
+      for (int b = lane; b < p.B; b += 32)
+        if (__ldg(p.lengths + b) > p.max_keys && p.status) atomicOr(p.status, SISA_ST_BAD_POS);
+    }
+    if (w < nwork) {
+      const int64_t x0 = run_start(w, tiles);
+      count = run_start(w + 1, tiles) - x0;
+      in = find_tile(p, x0);
+    }
   }
+  at = in;
   // the pieces this warp leaves for the CTA's merge: [0] of the unit that began before its run (s_ends: and
   // ends in it), [1] of the one that goes on after it; s_unit -1: none
   __shared__ int64_t s_unit[NW][2];
   __shared__ bool s_ends[NW];
+  __shared__ float s_lse;
+  __shared__ float s_x[kScores && kUnit ? UNIT_KEYS : 1];
   float* pieces = reinterpret_cast<float*>(gbase + OFF_REC);
   if (lane == 0) { s_unit[warp][0] = s_unit[warp][1] = -1; s_ends[warp] = false; }
   __syncwarp();
-  const int64_t x0 = w < nwork ? run_start(w, tiles) : 0, count = w < nwork ? run_start(w + 1, tiles) - x0 : 0;
 
   // ---- this lane's part of a tile's copies: operand op of the tile's sub-tile sub (pages of 16 slots
   // give a tile two sub-tiles)
@@ -233,9 +257,6 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
   const bool copier = sub < nsub && row_bytes > 0;
   const uint32_t key_bytes = 128 + 128 + 64 + 4 + (p.f_q ? 4 : 0);
 
-  Cursor in{}, at;
-  if (count > 0) in = find_tile(p, x0);
-  at = in;
   // the page of this lane's sub-tile at the fill cursor, read one tile ahead of its use
   auto page_at = [&]() {
     const int64_t j = in.t * TK + sub * rows_max;
@@ -317,7 +338,9 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
     float x = fmaf(reduce_scatter8(qk, part), c1, lam2 * (dec * reduce_scatter8(cb, part)));
     x = (mask >> key) & 1 ? fmaf(fq - fj, kLOG2E, x) : -INFINITY;
     if constexpr (kScores) {
-      if (at.t * TK + key < at.n) p.scores[((int64_t)at.b * p.H + at.h) * p.max_keys + at.t * TK + key] = x;
+      const int64_t j = at.t * TK + key;
+      if (kUnit) s_x[j] = x;
+      else if (j < at.n) p.scores[((int64_t)at.b * p.H + at.h) * p.max_keys + j] = x;
     }
     if (__any_sync(0xffffffffu, x > m_ref + 8.f)) {
       float mx = x;
@@ -377,6 +400,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
           reinterpret_cast<uint4*>(p.y + 2 * (at.b * p.y_sb + at.h * p.y_sh))[part] = o;
         }
         if (lane == 0) {
+          if (kUnit) s_lse = lse;
           p.lse_all[bh] = lse;
           if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
         }
@@ -404,14 +428,15 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
   // ---- the CTA's runs are neighbours: one warp merges their pieces in order. What began before the CTA or
   // goes on after it becomes its record 0 or 1.
   __syncthreads();
-  if (warp != 0) return;
+  if (!kUnit && warp != 0) return;
   Sum sum;
   int64_t unit = -1;                            // the unit being merged, -1: none
   bool before = false;                          // it began before this CTA
   auto close = [&](bool ends) {
     if (ends && !before) {
-      write_row<kHalf>(p, unit, sum);
-    } else {
+      const float lse = write_row<kHalf>(p, unit, sum);
+      if (kUnit && lane == 0) s_lse = lse;
+    } else if (!kUnit) {                        // (a unit's own CTA leaves pieces only when a wait ran out)
       float* rec = p.records + ((int64_t)blockIdx.x * 2 + (before ? 0 : 1)) * REC;
       if (lane == 0) *reinterpret_cast<float2*>(rec) = make_float2(sum.m, sum.l);
       *reinterpret_cast<float2*>(rec + 4 + 2 * lane) = sum.a;
@@ -419,7 +444,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
     unit = -1;
   };
 #pragma unroll 1
-  for (int i = 0; i < NW; ++i) {
+  for (int i = 0; i < NW && warp == 0; ++i) {
     if (s_unit[i][0] >= 0) {
       if (unit < 0) { unit = s_unit[i][0]; before = true; sum.clear(); }
       sum.add(pieces + (i * 2) * REC);
@@ -433,6 +458,22 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
     }
   }
   if (unit >= 0) close(false);
+  if constexpr (kUnit) {
+    const int64_t b = blockIdx.x / p.H, h = blockIdx.x % p.H, n = keys_of(p, (int)b);
+    if (n == 0 && warp == 0) {                  // a row with no keys
+      reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = 0u;
+      if (lane == 0) p.lse_all[blockIdx.x] = -INFINITY;
+    }
+    if constexpr (kScores) {
+      __syncthreads();
+      for (int64_t j = threadIdx.x; j < n; j += NW * 32) {
+        const int page = page_of(p.pg, (int)b, j, nullptr);
+        if (page < 0) continue;
+        const int64_t slot = page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
+        p.weight_out[slot] = p.pg.weight[slot] + exp2f(s_x[j] - s_lse);
+      }
+    }
+  }
 }
 
 // The records of one unit, merged by the JW warps of a block: each takes a run of them (the maximum first,
@@ -572,9 +613,19 @@ cudaError_t launch_after(K kernel, dim3 grid, int threads, cudaStream_t st, cons
 
 template <bool kHalf>
 cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
-  auto* main = p.weight_out ? paged_attn_kernel<kHalf, true> : paged_attn_kernel<kHalf, false>;
+  // Short tables: one launch and no join. 16 heads, one CTA per unit against the split (us, without / with
+  // weights): 1 x 256 keys 10.3 / 12.3 against 15.4 / 15.4, 8 x 256 12.3 / 14.2 against 18.5 / 19.5, 64 x 256
+  // 32.8 / 36.9 against 33.9 / 35.9; at 1024 keys 1 x 18.4 / 21.3 against 15.4 / 17.5, 64 x 69.6 / 84.0 against
+  // 72.7 / 74.9.
+  const bool unit = p.max_keys <= UNIT_KEYS;
+  auto* main = p.weight_out ? (unit ? paged_attn_kernel<kHalf, true, true> : paged_attn_kernel<kHalf, true, false>)
+                            : (unit ? paged_attn_kernel<kHalf, false, true> : paged_attn_kernel<kHalf, false, false>);
   cudaError_t e = cudaFuncSetAttribute(main, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
   if (e != cudaSuccess) return e;
+  if (unit) {
+    main<<<p.B * p.H, NW * 32, SMEM_BYTES, st>>>(p);
+    return cudaGetLastError();
+  }
   main<<<NCTA, NW * 32, SMEM_BYTES, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int units = p.B * p.H;

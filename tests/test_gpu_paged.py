@@ -53,6 +53,11 @@ def make_table(lengths, S, seed, dev):
     return table.to(dev), total
 
 
+def widen(table, columns=300):
+    """The table with further entries that name no page (they may not be read)."""
+    return torch.cat([table, torch.full((table.shape[0], columns), -7, dtype=torch.int32, device=table.device)], dim=1)
+
+
 def put(plane, table, b, values):
     """values (H, n, ...) into the first n slots of sequence b."""
     S, n = plane.shape[2], values.shape[1]
@@ -155,13 +160,17 @@ def check_attn(pages, table, rows, lengths, x, dev, accumulate=True):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("S", [16, 32, 64, 128, 256])
-def test_attention_lengths_around_pages_and_tiles(cuda_dev, S, dtype):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_lengths_around_pages_and_tiles(cuda_dev, S, dtype, wide):
+    """``wide``: the same sequences under a table for many more keys (its further entries, which no length
+    reaches, name no page): the kernels that split the keys serve them instead of the one-CTA-per-row kernel."""
     lengths = [1, 0, 2, S - 1, S, S + 1, 31, 32, 33, 63, 64, 65, 2 * S + 7, 300]
     pages, table, rows, x = attn_case(lengths, 3, S, dtype, cuda_dev, seed=S)
-    check_attn(pages, table, rows, lengths, x, cuda_dev)
+    check_attn(pages, widen(table) if wide else table, rows, lengths, x, cuda_dev)
 
 
-@pytest.mark.parametrize("B,H,n,S", [(1, 1, 1, 64), (1, 8, 5003, 64), (1, 1, 20011, 16), (7, 5, 777, 32), (40, 2, 129, 128)])
+@pytest.mark.parametrize("B,H,n,S", [(1, 1, 1, 64), (1, 8, 5003, 64), (1, 1, 20011, 16), (7, 5, 777, 32), (40, 2, 129, 128),
+                                     (3, 4, 512, 64), (3, 4, 513, 64), (33, 3, 1500, 256)])
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_attention_shapes(cuda_dev, B, H, n, S, accumulate):
     gen = torch.Generator().manual_seed(n)
@@ -175,8 +184,9 @@ def test_attention_large_scores_strong_forgetting_and_no_forget_gate(cuda_dev):
     lengths = [513, 40, 1, 900]
     for kw in (dict(qscale=30.0, frate=3.0), dict(forget=False)):
         pages, table, rows, x = attn_case(lengths, 4, 64, torch.bfloat16, cuda_dev, seed=9, **kw)
-        y, lse = run_attn(pages, table, lengths, x, cuda_dev)
-        for i, (yr, lr, p) in enumerate(attn_truth(rows, lengths, x)):
+        truth = attn_truth(rows, lengths, x)
+        for i, (yr, lr, p), t in ((i, r, t) for t in (table, widen(table)) for i, r in enumerate(truth)):
+            y, lse = run_attn(pages, t, lengths, x, cuda_dev)
             # scores of magnitude 2^10 are off by up to 2^-24 x 2^10 x a few in their fp32 sums
             assert max_abs(lse[i], lr) <= 2e-3
             assert bool(((y[i, :, 0].double().cpu() - yr).abs() <= HALF_ULP[y.dtype] * yr.abs() + 8e-3).all())
@@ -184,15 +194,19 @@ def test_attention_large_scores_strong_forgetting_and_no_forget_gate(cuda_dev):
 
 def test_attention_all_idle_and_minus_infinity_keys(cuda_dev):
     pages, table, rows, x = attn_case([0, 0], 2, 32, torch.bfloat16, cuda_dev, seed=1)
-    y, lse = run_attn(pages, table, [0, 0], x, cuda_dev, accumulate=True)
-    assert bool((y == 0).all()) and bool((lse == -math.inf).all())
+    for t in (table, widen(table)):
+        y, lse = run_attn(pages, t, [0, 0], x, cuda_dev, accumulate=True)
+        assert bool((y == 0).all()) and bool((lse == -math.inf).all())
     # a key whose score is -inf has no share, wherever it lies; whole tiles of them too
     lengths = [200]
     pages, table, rows, x = attn_case(lengths, 2, 32, torch.bfloat16, cuda_dev, seed=2)
     rows[0]["f"][:, :70] = math.inf
     rows[0]["f"][:, 133] = math.inf
     put(pages.f, table, 0, rows[0]["f"])
+    before = pages.weight.clone()
     check_attn(pages, table, rows, lengths, x, cuda_dev)
+    pages.weight.copy_(before)
+    check_attn(pages, widen(table), rows, lengths, x, cuda_dev)
 
 
 def test_attention_nan_key_reaches_output_and_status(cuda_dev):
@@ -200,8 +214,9 @@ def test_attention_nan_key_reaches_output_and_status(cuda_dev):
     pages, table, rows, x = attn_case(lengths, 2, 64, torch.bfloat16, cuda_dev, seed=3)
     rows[0]["g"][1, 77] = math.nan
     put(pages.g, table, 0, rows[0]["g"])
-    with pytest.raises(FloatingPointError):
-        run_attn(pages, table, lengths, x, cuda_dev)
+    for t in (table, widen(table)):
+        with pytest.raises(FloatingPointError):
+            run_attn(pages, t, lengths, x, cuda_dev)
     from sisa_b200 import backends
 
     mode = backends.get_check_mode()
@@ -261,13 +276,12 @@ def test_attention_pages_past_32_bit_offsets(cuda_dev):
 def test_attention_bad_table_and_length_set_the_status(cuda_dev):
     lengths = [128, 50]
     pages, table, rows, x = attn_case(lengths, 2, 32, torch.bfloat16, cuda_dev, seed=6)
-    bad = table.clone()
-    bad[0, 1] = pages.n_pages
-    with pytest.raises(ValueError):
-        run_attn(pages, bad, lengths, x, cuda_dev, accumulate=True)
-    bad[0, 1] = -1
-    with pytest.raises(ValueError):
-        run_attn(pages, bad, lengths, x, cuda_dev)
+    for page, wide in ((pages.n_pages, False), (-1, False), (pages.n_pages, True), (-1, True)):
+        bad = widen(table) if wide else table.clone()
+        bad[0, 1] = page
+        for acc in (True, False):
+            with pytest.raises(ValueError):
+                run_attn(pages, bad, lengths, x, cuda_dev, accumulate=acc)
     with pytest.raises(ValueError):
         run_attn(pages, table, [129, 50], x, cuda_dev)
 
