@@ -4,6 +4,7 @@
 ``sisa_fused(proj, z, lam, n_head) -> y``, ``fused_layout``, ``concat_fused_weights``   (:mod:`.fused`)
 ``linear_cross_entropy(hidden, weight, labels, ignore_index=-100)``   (:mod:`.linear_ce`)
 ``decode_attention(...)``   (:mod:`.decode`)
+``KeyPages``, ``paged_attention``, ``paged_evict``, ``paged_append``, ``attention_key_weights``, ``paged_fill``   (:mod:`.paged`)
 
 Submodules load on first attribute access.
 """
@@ -12,7 +13,8 @@ from __future__ import annotations
 import importlib
 
 __all__ = ["sisa_attention_cuda", "sisa_fused", "fused_layout", "concat_fused_weights", "linear_cross_entropy",
-           "decode_attention"]
+           "decode_attention", "KeyPages", "paged_attention", "paged_evict", "paged_append", "attention_key_weights",
+           "paged_fill"]
 
 _LAZY = {
     "sisa_attention_cuda": "attention",
@@ -21,6 +23,12 @@ _LAZY = {
     "concat_fused_weights": "fused",
     "linear_cross_entropy": "linear_ce",
     "decode_attention": "decode",
+    "KeyPages": "paged",
+    "paged_attention": "paged",
+    "paged_evict": "paged",
+    "paged_append": "paged",
+    "attention_key_weights": "paged",
+    "paged_fill": "paged",
 }
 
 
