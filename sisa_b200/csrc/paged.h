@@ -80,7 +80,7 @@ int64_t paged_attn_workspace_floats(int64_t units, int64_t max_keys, bool scores
 cudaError_t launch_paged_attn(PagedAttnParams p, int dtype, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictParams& p, cudaStream_t st);
 cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, cudaStream_t st);
-cudaError_t launch_paged_fill(const PagedFillParams& p, cudaStream_t st);
+cudaError_t launch_paged_fill(PagedFillParams p, cudaStream_t st);
 
 // The page that holds slots [j, ...) of sequence b, or -1 (and SISA_ST_BAD_POS) if the table's entry names
 // no page of the pool.

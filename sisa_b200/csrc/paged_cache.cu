@@ -227,10 +227,6 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
   const uint32_t below = (1u << lane) - 1;
   int32_t* out = p.index + (int64_t)bh * p.keep;
   const int L = (int)p.L, old = (int)(p.L - p.recent);   // positions [0, old) compete for keep - recent places
-  if (p.keep == p.L) {
-    for (int j = tid; j < L; j += ST) out[j] = j;
-    return;
-  }
   const float* wt = p.weight + (int64_t)bh * p.L;
   const bool in_smem = old <= SEL_SMEM;
   if (in_smem) {
@@ -354,7 +350,7 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
       waited = true;
     }
     if (page >= 0) {
-      const int64_t j = index[r], in = r & ((1 << p.pg.page_shift) - 1);
+      const int64_t j = p.index ? index[r] : r, in = r & ((1 << p.pg.page_shift) - 1);
       const uint4 k = __ldg(reinterpret_cast<const uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + j * p.k_sl)) + part);
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.v + 2 * (b * p.v_sb + h * p.v_sh + j * p.v_sl)) + part);
       uint4 m = make_uint4(0, 0, 0, 0);
@@ -364,7 +360,7 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
       if (part < 4) reinterpret_cast<uint4*>(p.pg.b + 2 * (page * p.pg.b_sp + h * p.pg.b_sh + in * 32))[part] = m;
     }
     if (tid < GK && r0 + tid < p.keep) {
-      const int64_t rr = r0 + tid, j = index[rr];
+      const int64_t rr = r0 + tid, j = p.index ? index[rr] : rr;
       const int pp = page_of(p.pg, b, rr, nullptr);
       if (pp >= 0) {
         const int64_t at = pp * p.pg.s_sp + h * p.pg.s_sh + (rr & ((1 << p.pg.page_shift) - 1));
@@ -407,16 +403,21 @@ cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, cudaStrea
   return cudaGetLastError();
 }
 
-cudaError_t launch_paged_fill(const PagedFillParams& p, cudaStream_t st) {
-  const int64_t old = p.L - p.recent;
-  const size_t smem = p.keep < p.L && old <= pca::SEL_SMEM ? (size_t)old * 4 : 0;
-  cudaError_t e = cudaFuncSetAttribute(pca::paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       pca::SEL_SMEM * 4);
-  if (e != cudaSuccess) return e;
-  pca::paged_select_kernel<<<p.B * p.H, pca::ST, smem, st>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
+cudaError_t launch_paged_fill(PagedFillParams p, cudaStream_t st) {
+  const bool choose = p.keep < p.L;
+  if (choose) {
+    const int64_t old = p.L - p.recent;
+    const size_t smem = old <= pca::SEL_SMEM ? (size_t)old * 4 : 0;
+    cudaError_t e = cudaFuncSetAttribute(pca::paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         pca::SEL_SMEM * 4);
+    if (e != cudaSuccess) return e;
+    pca::paged_select_kernel<<<p.B * p.H, pca::ST, smem, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  } else {
+    p.index = nullptr;                           // every key is kept: slot r takes position r
+  }
   const int64_t chunks = (p.keep + pca::GK - 1) / pca::GK;
+  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.B * p.H, (unsigned)(chunks < 65535 ? chunks : 65535));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
@@ -424,7 +425,7 @@ cudaError_t launch_paged_fill(const PagedFillParams& p, cudaStream_t st) {
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its blocks wait for the choice themselves
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = choose ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, pca::paged_gather_kernel, p);
 }
 
