@@ -388,7 +388,7 @@ typedef struct sisa_pages {
  * weight_out_j = weight_j + softmax(s)_j; slots past a sequence's length are not written. A sequence of
  * length <= 0 gives y = 0 and lse = -inf; a length above max_pages * page_size is cut there and sets
  * SISA_ST_BAD_POS. workspace: sisa_paged_attn_workspace(B, H, max_pages * page_size, weight_out != NULL)
- * bytes, 16-byte aligned, one call at a time. Deterministic. */
+ * bytes, 16-byte aligned, one call at a time (NULL where that is 0: short tables). Deterministic. */
 int64_t sisa_paged_attn_workspace(int64_t B, int64_t H, int64_t max_keys, int accumulate);
 int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, const float* f_q,
                     const sisa_pages* pages, const int32_t* table, int64_t table_sb, int64_t max_pages,

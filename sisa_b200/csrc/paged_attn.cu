@@ -178,7 +178,7 @@ __device__ __forceinline__ float write_row(const PagedAttnParams& p, int64_t bh,
   const float lse = s.m + log2f(s.l), r = 1.f / s.l;
   reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = pack2<kHalf>(s.a.x * r, s.a.y * r);
   if (lane == 0) {
-    p.lse_all[bh] = lse;
+    if (p.lse_all) p.lse_all[bh] = lse;
     if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
   }
   return lse;
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
         }
         if (lane == 0) {
           if (kUnit) s_lse = lse;
-          p.lse_all[bh] = lse;
+          if (!kUnit || p.lse_all) p.lse_all[bh] = lse;
           if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
         }
       } else {
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
     const int64_t b = blockIdx.x / p.H, h = blockIdx.x % p.H, n = keys_of(p, (int)b);
     if (n == 0 && warp == 0) {                  // a row with no keys
       reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = 0u;
-      if (lane == 0) p.lse_all[blockIdx.x] = -INFINITY;
+      if (lane == 0 && p.lse_all) p.lse_all[blockIdx.x] = -INFINITY;
     }
     if constexpr (kScores) {
       __syncthreads();
@@ -638,15 +638,19 @@ cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
 }  // namespace pat
 
 int64_t paged_attn_workspace_floats(int64_t units, int64_t max_keys, bool scores) {
+  if (max_keys <= pat::UNIT_KEYS) return 0;      // one CTA per unit: nothing passes between kernels
   const int64_t base = (int64_t)pat::NCTA * 2 * pat::REC + ((units + 3) & ~int64_t(3));
   return base + (scores ? units * max_keys : 0);
 }
 
 cudaError_t launch_paged_attn(PagedAttnParams p, int dtype, cudaStream_t st) {
   const int64_t units = (int64_t)p.B * p.H;
-  p.records = p.ws;
-  p.lse_all = p.lse ? p.lse : p.ws + (int64_t)pat::NCTA * 2 * pat::REC;
-  p.scores = p.ws + paged_attn_workspace_floats(units, 0, false);
+  p.lse_all = p.lse;
+  if (p.ws) {
+    p.records = p.ws;
+    if (!p.lse) p.lse_all = p.ws + (int64_t)pat::NCTA * 2 * pat::REC;
+    p.scores = p.ws + paged_attn_workspace_floats(units, p.max_keys, false);
+  }
   return dtype == 1 ? pat::launch<true>(p, st) : pat::launch<false>(p, st);
 }
 

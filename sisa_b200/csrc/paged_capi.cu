@@ -82,7 +82,10 @@ int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, 
   if ((rc = sisa::capi_check_view(q, 2, "q")) || (rc = sisa::capi_check_view(c, 2, "c")) ||
       (rc = sisa::capi_check_view(y, 2, "y")))
     return rc;
-  if (!g_q || !lengths || !lam || !workspace) return fail(SISA_ERR_VALUE, what, "null pointer");
+  const int64_t max_keys = max_pages * pages->page_size;
+  if (!g_q || !lengths || !lam) return fail(SISA_ERR_VALUE, what, "null pointer");
+  const bool needs_ws = sisa::paged_attn_workspace_floats(B * H, max_keys, false) > 0;
+  if (needs_ws && !workspace) return fail(SISA_ERR_VALUE, what, "null workspace");
   if (f_q && !pages->f) return fail(SISA_ERR_VALUE, what, "f_q is given but the pages hold no f");
   if (weight_out && !pages->weight) return fail(SISA_ERR_VALUE, what, "weight_out is given but the pages hold no weight");
   if (!aligned(workspace, 16) || !aligned(weight_out, 16))
@@ -91,8 +94,8 @@ int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, 
   p.c = static_cast<const char*>(c->data); p.c_sb = c->stride_b; p.c_sh = c->stride_h;
   p.g_q = g_q; p.f_q = f_q; p.lengths = lengths; p.lam = lam;
   p.y = static_cast<char*>(y->data); p.y_sb = y->stride_b; p.y_sh = y->stride_h;
-  p.lse = lse; p.weight_out = weight_out; p.ws = static_cast<float*>(workspace);
-  p.B = (int)B; p.H = (int)H; p.max_keys = max_pages * pages->page_size;
+  p.lse = lse; p.weight_out = weight_out; p.ws = needs_ws ? static_cast<float*>(workspace) : nullptr;
+  p.B = (int)B; p.H = (int)H; p.max_keys = max_keys;
   p.status = status;
   return launched(sisa::launch_paged_attn(p, dtype, static_cast<cudaStream_t>(stream)), what);
 }

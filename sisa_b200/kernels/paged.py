@@ -67,6 +67,7 @@ class KeyPages:
                              _lib.ptr(token), k.stride(0), k.stride(1), v.stride(0), v.stride(1), b.stride(0), b.stride(1),
                              g.stride(0), g.stride(1), P, S)
         self.cbytes = bytes(c)                  # the struct every call passes
+        self.ws_bytes: dict[tuple, int] = {}    # workspace sizes of the tables seen
 
     @classmethod
     def empty(cls, n_pages: int, n_head: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda",
@@ -169,10 +170,17 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
     fq = None if fgate is None else _f32(fgate)
     y = q.new_empty((B, H, 1, 64))              # (new_empty costs less host time than torch.empty with a device)
     lse = lam.new_empty((B, H)) if return_lse else None
-    ws = lam.new_empty(lib.sisa_paged_attn_workspace(B, H, mp * pages.page_size, accumulate) // 4)
+    key = (B, mp, accumulate)
+    nbytes = pages.ws_bytes.get(key)
+    if nbytes is None:
+        if len(pages.ws_bytes) >= 1024:         # a long-running process with ever-changing tables
+            pages.ws_bytes.clear()
+        nbytes = pages.ws_bytes[key] = lib.sisa_paged_attn_workspace(B, H, mp * pages.page_size, accumulate)
+    ws = lam.new_empty(nbytes // 4) if nbytes else None
     rc = lib.sisa_paged_attn(_lib.view4_bytes(q), _lib.view4_bytes(c), gq.data_ptr(), None if fq is None else fq.data_ptr(),
                              pages.cbytes, tp, tsb, mp, lp, lam.data_ptr(), B, H, pages.dtype_code, _lib.view4_bytes(y),
-                             None if lse is None else lse.data_ptr(), None if wo is None else wo.data_ptr(), ws.data_ptr(),
+                             None if lse is None else lse.data_ptr(), None if wo is None else wo.data_ptr(),
+                             None if ws is None else ws.data_ptr(),
                              backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_attn")
     backends.after_call(dev)

@@ -57,7 +57,7 @@ def test_pages_and_attention_refusals():
                    (dict(b_sh=16 * 64), V), (dict(s_sh=32), V), (dict(s_sp=130), AL), (dict(f=None), V), (dict(v_sp=-8192), V)):
         assert attn(pages(**kw)) == rc, kw
     for kw, rc in ((dict(dtype=_lib.F32), T), (dict(B=0), V), (dict(B=65536), V), (dict(table=None), V), (dict(tsb=3), V),
-                   (dict(mp=0), V), (dict(lengths=None), V), (dict(ws=None), V), (dict(ws=A + 4), AL), (dict(wo=A + 4), AL),
+                   (dict(mp=0), V), (dict(lengths=None), V), (dict(ws=None, mp=16, tsb=16), V), (dict(ws=A + 4), AL), (dict(wo=A + 4), AL),
                    (dict(gq=None), V), (dict(lam=None), V), (dict(q=_lib.View4(A + 8, 128, 64, 64)), AL),
                    (dict(y=_lib.View4(None, 128, 64, 64)), V)):
         assert attn(pages(), **kw) == rc, kw
