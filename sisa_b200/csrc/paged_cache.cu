@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) 
 //      are written in order.
 // The weights of up to SEL_SMEM keys are ordered once into shared memory; longer prompts are read again
 // from L2 in each pass.
-constexpr int ST = 1024, SEL_SMEM = 40960;
+constexpr int ST = 1024, SW = ST / 32, SEL_SMEM = 40960;
+static_assert(SW <= 32 && 2048 % ST == 0, "scan and bins");
 constexpr int BINS = 2048;
 
 // Exclusive scan over the block's threads; total in every thread.
@@ -202,7 +203,7 @@ __device__ __forceinline__ int scan_excl(int v, int* s_warp, int& total) {
   }
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
-  const int c = s_warp[lane];                    // ST / 32 == 32 warps
+  const int c = lane < SW ? s_warp[lane] : 0;
   int y = c;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -259,18 +260,18 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
         }
       }
       __syncthreads();
-      // thread t holds the bins 2047 - 2t and 2046 - 2t: the scan runs from the largest digit down
-      const int d = BINS - 1 - 2 * tid, h0 = s_hist[d], h1 = s_hist[d - 1];
-      int total;
-      const int over = scan_excl(h0 + h1, s_warp, total);
-      if (over < left && left <= over + h0) {
-        s_digit = d;
+      // thread t holds BINS / ST bins from BINS - 1 - t BINS / ST down: the scan runs from the largest digit
+      const int d = BINS - 1 - (BINS / ST) * tid;
+      int own = 0, total;
+#pragma unroll
+      for (int i = 0; i < BINS / ST; ++i) own += s_hist[d - i];
+      int over = scan_excl(own, s_warp, total);
+      if (over < left && left <= over + own) {   // the wanted digit is one of this thread's
+        int i = 0;
+        while (left > over + s_hist[d - i]) over += s_hist[d - i++];
+        s_digit = d - i;
         s_left = left - over;
-        s_in = h0;
-      } else if (over + h0 < left && left <= over + h0 + h1) {
-        s_digit = d - 1;
-        s_left = left - over - h0;
-        s_in = h1;
+        s_in = s_hist[d - i];
       }
       __syncthreads();
       prefix |= s_digit << shift;
@@ -290,7 +291,8 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
           int at = 0;
           if (lane == 0 && m) at = atomicAdd(&s_count, __popc(m));
           at = __shfl_sync(0xffffffffu, at, 0);
-          if (is) s_buf[at + __popc(m & below)] = u;
+          at += __popc(m & below);
+          if (is && at < 4 * ST) s_buf[at] = u;
         }
         cand = in;
       }
@@ -304,9 +306,9 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
   int* s_before = reinterpret_cast<int*>(s_buf + 3 * ST);
   int done = 0, ties = 0;                        // kept, and keys at T, in the chunks before
   for (int j0 = 0; j0 < L; j0 += ST * 32) {
-    // group g of the chunk holds 32 consecutive positions, a warp every 32nd group
+    // group g of the chunk holds 32 consecutive positions
     const int groups = min(ST, (L - j0 + 31) / 32);
-    for (int g = warp; g < groups; g += 32) {
+    for (int g = warp; g < groups; g += SW) {
       const int j = j0 + g * 32 + lane;
       const uint32_t u = j < old ? key_at(j) : 0u;
       const uint32_t sure = __ballot_sync(0xffffffffu, j < L && (j >= old || u > prefix));
@@ -317,15 +319,15 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
     int tot_tie, tot;
     const int nt = tid < groups ? __popc(s_tie[tid]) : 0, ns = tid < groups ? __popc(s_sure[tid]) : 0;
     const int tb = ties + scan_excl(nt, s_warp, tot_tie);
-    const int at = done + scan_excl(ns + max(0, min(nt, left - tb)), s_warp, tot);
-    s_base[tid] = at;
+    s_base[tid] = done + scan_excl(ns + max(0, min(nt, left - tb)), s_warp, tot);
     s_before[tid] = tb;
     __syncthreads();
-    for (int g = warp; g < groups; g += 32) {
+    for (int g = warp; g < groups; g += SW) {
       const uint32_t sure = s_sure[g], tie = s_tie[g];
       const bool keep = ((sure >> lane) & 1) || (((tie >> lane) & 1) && s_before[g] + __popc(tie & below) < left);
       const uint32_t kept = tie ? __ballot_sync(0xffffffffu, keep) : sure;
-      if (keep) out[s_base[g] + __popc(kept & below)] = j0 + g * 32 + lane;
+      const int at = s_base[g] + __popc(kept & below);
+      if (keep && at < (int)p.keep) out[at] = j0 + g * 32 + lane;
     }
     __syncthreads();
     done += tot;
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(ST) paged_select_kernel(PagedFillParams p) {
 // read the same part of the prompt for all heads, whose rows lie side by side in the projection. (Two keys
 // a lane: 101 instead of 97 us for 16 x 16 units of 8192 -> 2048 keys, four: 122 us.)
 constexpr int GK = 32;
-__global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
+__global__ void __launch_bounds__(256, 8) paged_gather_kernel(PagedFillParams p) {
   const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, tid = threadIdx.x, part = tid & 7;
   const int32_t* index = p.index + (int64_t)bh * p.keep;
   bool waited = false;
@@ -349,8 +351,9 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
       asm volatile("griddepcontrol.wait;" ::: "memory");
       waited = true;
     }
-    if (page >= 0) {
-      const int64_t j = p.index ? index[r] : r, in = r & ((1 << p.pg.page_shift) - 1);
+    const int j = page < 0 ? -1 : (p.index ? index[r] : (int)r);
+    if ((unsigned)j < (unsigned)p.L) {           // (an index outside the prompt cannot arise; it would be left out)
+      const int64_t in = r & ((1 << p.pg.page_shift) - 1);
       const uint4 k = __ldg(reinterpret_cast<const uint4*>(p.k + 2 * (b * p.k_sb + h * p.k_sh + j * p.k_sl)) + part);
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.v + 2 * (b * p.v_sb + h * p.v_sh + j * p.v_sl)) + part);
       uint4 m = make_uint4(0, 0, 0, 0);
@@ -360,9 +363,9 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
       if (part < 4) reinterpret_cast<uint4*>(p.pg.b + 2 * (page * p.pg.b_sp + h * p.pg.b_sh + in * 32))[part] = m;
     }
     if (tid < GK && r0 + tid < p.keep) {
-      const int64_t rr = r0 + tid, j = p.index ? index[rr] : rr;
-      const int pp = page_of(p.pg, b, rr, nullptr);
-      if (pp >= 0) {
+      const int64_t rr = r0 + tid;
+      const int j = p.index ? index[rr] : (int)rr, pp = page_of(p.pg, b, rr, nullptr);
+      if (pp >= 0 && (unsigned)j < (unsigned)p.L) {
         const int64_t at = pp * p.pg.s_sp + h * p.pg.s_sh + (rr & ((1 << p.pg.page_shift) - 1));
         const float g = __ldg(p.g + b * p.g_sb + h * p.g_sh + j);
         const float f = p.f ? __ldg(p.f + b * p.f_sb + h * p.f_sh + j) : 0.f;
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(256) paged_gather_kernel(PagedFillParams p) {
         p.pg.g[at] = g;
         if (p.pg.f) p.pg.f[at] = f;
         if (p.pg.weight) p.pg.weight[at] = w;
-        if (p.pg.token) p.pg.token[at] = (int)j;
+        if (p.pg.token) p.pg.token[at] = j;
       }
     }
   }
