@@ -168,7 +168,7 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
         c = c.to(q.dtype)
     q, c, gq, lam = _operand(q), _operand(c), _f32(g), _f32(lam)
     fq = None if fgate is None else _f32(fgate)
-    y = q.new_empty((B, H, 1, 64))              # (new_empty costs less host time than torch.empty with a device)
+    y = torch.empty_like(q)                     # (less host time than torch.empty with a device)
     lse = lam.new_empty((B, H)) if return_lse else None
     key = (B, mp, accumulate)
     nbytes = pages.ws_bytes.get(key)
@@ -249,7 +249,7 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
         if z.numel() != B * H or z.device != dev:
             raise ValueError(f"z must be ({B}, 1, {H}) on {dev}, got {tuple(z.shape)} on {z.device}")
         z2 = _f32(z)
-        f = carry.new_empty((B, H, 1))
+        f = torch.empty_like(g)
         zp, fp = z2.data_ptr(), f.data_ptr()
     rc = _lib.load().sisa_paged_append(proj.data_ptr(), sb if B > 1 else width, zp, H, pages.cbytes, tp, tsb, mp, pp, sp,
                                        int(budget or 0), B, H, pages.dtype_code, carry.data_ptr(), co.data_ptr(),
