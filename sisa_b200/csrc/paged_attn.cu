@@ -481,16 +481,30 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
   }
 }
 
+constexpr int JW = 8;
+// The CTAs that hold pieces of unit (b, h), found by warp 0 from the lengths alone, then (every thread) the end
+// of the kernel that writes the records.
+__device__ __forceinline__ int2 unit_span(const PagedAttnParams& p, int b, int h, int64_t n) {
+  __shared__ int s_span[2];
+  if (threadIdx.x < 32) {
+    int64_t all;
+    const int64_t T = (n + TK - 1) / TK, u0 = tiles_before(p, b, all) * p.H + h * T, tiles = all * p.H;
+    if (threadIdx.x == 0) {
+      s_span[0] = T == 0 ? 0 : worker_of(u0, tiles) / NW;
+      s_span[1] = T == 0 ? 0 : worker_of(u0 + T - 1, tiles) / NW;
+    }
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __syncthreads();
+  return make_int2(s_span[0], s_span[1]);
+}
+
 // The records of one unit, merged by the JW warps of a block: each takes a run of them (the maximum first,
 // then every record on its own, so that the loads are in flight together), and warp 0 the runs' sums, all in
 // CTA order. Returns false (to every warp) for a unit that one CTA finished or that has no keys; the sum is
 // warp 0's.
-constexpr int JW = 8;
-__device__ __forceinline__ bool join_unit(const PagedAttnParams& p, int b, int h, int64_t n, Sum& sum) {
-  int64_t all;
-  const int64_t T = (n + TK - 1) / TK, u0 = tiles_before(p, b, all) * p.H + h * T, tiles = all * p.H;
-  if (T == 0) return false;
-  const int c0 = worker_of(u0, tiles) / NW, c1 = worker_of(u0 + T - 1, tiles) / NW;
+__device__ __forceinline__ bool join_unit(const PagedAttnParams& p, int2 span, Sum& sum) {
+  const int c0 = span.x, c1 = span.y;
   if (c0 == c1) return false;
   __shared__ __align__(16) float s_sum[JW][REC];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -536,11 +550,10 @@ __device__ __forceinline__ void finish_unit(const PagedAttnParams& p, int64_t bh
 
 template <bool kHalf>
 __global__ void __launch_bounds__(JW * 32) paged_join_kernel(PagedAttnParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t bh = blockIdx.x;
   const int64_t n = keys_of(p, (int)(bh / p.H));
   Sum sum;
-  const bool joined = join_unit(p, (int)(bh / p.H), (int)(bh % p.H), n, sum);
+  const bool joined = join_unit(p, unit_span(p, (int)(bh / p.H), (int)(bh % p.H), n), sum);
   if (threadIdx.x < 32) finish_unit<kHalf>(p, bh, n, joined, sum);
 }
 
@@ -566,11 +579,11 @@ __global__ void __launch_bounds__(WT) paged_weights_kernel(PagedAttnParams p) {
   Four f;
   f.at = place(j);
   f.w = f.at >= 0 ? *reinterpret_cast<const float4*>(p.pg.weight + f.at) : make_float4(0.f, 0.f, 0.f, 0.f);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 span = unit_span(p, b, h, n);
   f.x = f.at >= 0 ? *reinterpret_cast<const float4*>(xs + j) : make_float4(0.f, 0.f, 0.f, 0.f);
   __shared__ float s_lse;
   Sum sum;
-  const bool joined = join_unit(p, b, h, n, sum);
+  const bool joined = join_unit(p, span, sum);
   if (threadIdx.x < 32) {
     if (blockIdx.x == 0) finish_unit<kHalf>(p, bh, n, joined, sum);
     if (threadIdx.x == 0 && n > 0) s_lse = joined ? sum.m + log2f(sum.l) : p.lse_all[bh];
