@@ -531,6 +531,98 @@ def test_fill_whole_prompt_without_weights_or_planes(cuda_dev):
     assert torch.equal(get(pages.v, table, 0, 90), v[0].cpu()) and torch.equal(get(pages.f, table, 0, 90), pos[0, :, 1, :90].cpu())
 
 
+@pytest.mark.parametrize("levels", [None, 3])
+@pytest.mark.parametrize("L,keep,recent", [(33000, 5000, 100), (70000, 9000, 0), (41000, 40999, 7)])
+def test_fill_long_prompts(cuda_dev, L, keep, recent, levels):
+    """Prompts past one chunk of the compaction and past the shared memory of the select; with ``levels`` the
+    weights take three values only, so that no digit tells the candidates apart."""
+    import numpy as np
+    from sisa_b200 import backends
+    from sisa_b200.kernels.paged import paged_fill
+
+    gen = torch.Generator().manual_seed(L + (levels or 0))
+    w = torch.rand(1, 2, L, generator=gen)
+    if levels:
+        w = (w * levels).floor() / levels
+    src = [torch.randn(1, 2, L, d, generator=gen).to(torch.bfloat16).to(cuda_dev) for d in (64, 64, 32)]
+    g, f = (torch.randn(1, 2, L, generator=gen).to(cuda_dev) for _ in range(2))
+    table, P = make_table([keep], 64, 1, cuda_dev)
+    pages = make_pages(P, 2, 64, torch.bfloat16, cuda_dev, fill=0.25)
+    paged_fill(pages, table, *src, g, f, weight=w.to(cuda_dev), keep=keep, recent=recent)
+    backends.check_status(cuda_dev)
+    old = L - recent
+    idx = []
+    for h in range(2):
+        top = np.lexsort((np.arange(old), -w[0, h, :old].numpy()))[:keep - recent]
+        idx.append(np.concatenate([np.sort(top), np.arange(old, L)]))
+    idx = torch.from_numpy(np.stack(idx))
+    assert torch.equal(get(pages.token, table, 0, keep).long(), idx)
+    for plane, x in ((pages.k, src[0]), (pages.v, src[1]), (pages.b, src[2])):
+        assert torch.equal(get(plane, table, 0, keep), x[0].cpu().gather(1, idx.unsqueeze(-1).expand(-1, -1, x.shape[-1])))
+    for plane, x in ((pages.g, g), (pages.f, f), (pages.weight, w)):
+        assert torch.equal(get(plane, table, 0, keep), x[0].cpu().gather(1, idx))
+
+
+def test_attention_of_many_tiles(cuda_dev):
+    """More tiles than one wave of warps takes (units spread over many CTAs, runs that cross units), against fp64
+    on the GPU, with and without weights."""
+    from sisa_b200 import backends
+    from sisa_b200.kernels.paged import KeyPages, paged_attention
+
+    dev, H, S, lengths = cuda_dev, 16, 128, [90001, 40, 0, 12345]
+    gen = torch.Generator(device=dev).manual_seed(1)
+    table, P = make_table(lengths, S, 2, dev)
+    rnd = lambda *shape: torch.randn(shape, generator=gen, device=dev)  # noqa: E731
+    pages = KeyPages(rnd(P, H, S, 64).half(), rnd(P, H, S, 64).half(), rnd(P, H, S, 32).half(), -rnd(P, H, S).abs(),
+                     -rnd(P, H, S).abs(), rnd(P, H, S).abs())
+    q, c = rnd(4, H, 1, 64).half(), rnd(4, H, 1, 32).half()
+    gq, fq, lam = -2 * torch.ones(4, H, 1, device=dev), -3 * torch.ones(4, H, 1, device=dev), torch.linspace(0.2, 1.0, H, device=dev)
+    ln = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    before = pages.weight.clone()
+    y0, l0 = paged_attention(q, c, gq, fq, pages, table, ln, lam, return_lse=True)
+    y, lse = paged_attention(q, c, gq, fq, pages, table, ln, lam, accumulate=True, return_lse=True)
+    backends.check_status(dev)
+    assert torch.equal(y, y0) and torch.equal(lse, l0)
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert bool((y[b] == 0).all()) and bool((lse[b] == -math.inf).all())
+            continue
+        j = torch.arange(n, device=dev)
+        pg, sl = table[b].long()[j // S], j % S
+        for h in range(H):
+            s = pages.k[pg, h, sl].double() @ q[b, h, 0].double() / 8
+            dec = torch.exp((gq[b, h].double() - pages.g[pg, h, sl].double()).clamp_max(0))
+            s = s + lam[h].double() * dec * (pages.b[pg, h, sl].double() @ c[b, h, 0].double()) + fq[b, h].double() - pages.f[pg, h, sl].double()
+            p = torch.softmax(s, 0)
+            want, v = p @ pages.v[pg, h, sl].double(), pages.v[pg, h, sl]
+            assert bool(((y[b, h, 0].double() - want).abs() <= 2.0 ** -11 * want.abs() + SHARE_REL * v.abs().max() + 2.0 ** -25).all())
+            assert abs(float(lse[b, h]) - float(torch.logsumexp(s, 0)) * LOG2E) <= 5e-5
+            ww = before[pg, h, sl].double() + p
+            assert bool(((pages.weight[pg, h, sl].double() - ww).abs() <= SHARE_REL * p + 2.0 ** -23 * ww + 1e-30).all())
+
+
+@pytest.mark.parametrize("L,first", [(5000, 0), (9001, 8000)])
+def test_key_weights_long_prompts(cuda_dev, L, first):
+    """Sums over thousands of queries, against fp64 on the GPU."""
+    from sisa_b200 import backends
+    from sisa_b200.kernels.paged import attention_key_weights
+
+    q, k, v, c, b, pos, lam, lse = prompt(1, 2, L, torch.bfloat16, cuda_dev, seed=L)
+    w = attention_key_weights(q, k, c, b, pos, lam, lse, first_query=first)
+    backends.check_status(cuda_dev)
+    want = torch.zeros(2, L, dtype=torch.float64, device=cuda_dev)
+    g, f = pos[0, :, 0, :L].double(), pos[0, :, 1, :L].double()
+    j = torch.arange(L, device=cuda_dev)
+    for h in range(2):
+        for i0 in range(first, L, 1000):
+            i = torch.arange(i0, min(L, i0 + 1000), device=cuda_dev)
+            s = q[0, h, i].double() @ k[0, h].double().t() / 8
+            s = s + lam[h].double() * torch.exp((g[h, i, None] - g[h, None]).clamp_max(0)) * (c[0, h, i].double() @ b[0, h].double().t())
+            s = s + f[h, i, None] - f[h, None] - lse[0, h, i, None].double() / LOG2E
+            want[h] += torch.exp(s).masked_fill(j[None] > i[:, None], 0.0).sum(0)
+    assert bool(((w[0].double() - want).abs() <= SHARE_REL * want + 1e-30).all())
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals(cuda_dev):
     from sisa_b200.kernels import paged as K
