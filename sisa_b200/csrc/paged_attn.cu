@@ -72,7 +72,7 @@ __device__ __forceinline__ int64_t tiles_before(const PagedAttnParams& p, int b,
 // The line is shared by one worker (warp) per tile while there are few tiles, then by the warps of one wave,
 // and beyond GRAIN tiles a worker by more whole waves, up to eight; none has an empty run. Worker w takes the
 // tiles [run_start(w), run_start(w + 1)); worker_of is its inverse.
-__device__ __forceinline__ int64_t workers(int64_t tiles) {
+__host__ __device__ __forceinline__ int64_t workers(int64_t tiles) {
   if (tiles < WMIN) return tiles;
   const int64_t waves = tiles / (WMIN * GRAIN);
   return waves < 1 ? WMIN : (waves < 8 ? waves * WMIN : NWORK);
@@ -644,7 +644,10 @@ cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
     main<<<p.B * p.H, NW * 32, SMEM_BYTES, st>>>(p);
     return cudaGetLastError();
   }
-  main<<<NCTA, NW * 32, SMEM_BYTES, st>>>(p);
+  // As many CTAs as the table could need (workers() never falls with the tiles): the lengths are only known on
+  // the device, and every CTA without work still costs its launch.
+  const int64_t most = workers((int64_t)p.B * p.H * ((p.max_keys + TK - 1) / TK));
+  main<<<(unsigned)((most + NW - 1) / NW), NW * 32, SMEM_BYTES, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int units = p.B * p.H;
   if (!p.weight_out) return launch_after(paged_join_kernel<kHalf>, dim3(units), JW * 32, st, p);
