@@ -61,14 +61,17 @@ __global__ void __launch_bounds__(NT) paged_evict_kernel(PagedEvictParams p) {
       f.ok = true;
       return f;
     };
+    // a thread meets its slots in ascending order, so the first of the least weight is kept by a strict
+    // comparison; 0xffffffff is above the order of every weight
+    uint32_t least = 0xffffffffu, slot = 0;
     auto take = [&](const Four& f, int64_t j) {
       if (!f.ok) return;
       const float w[4] = {f.w.x, f.w.y, f.w.z, f.w.w};
       const int t[4] = {f.t.x, f.t.y, f.t.z, f.t.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const unsigned long long key = ((unsigned long long)weight_order(w[e]) << 32) | (unsigned)(j + e);
-        if (j + e < p.budget && t[e] < newest && key < best) best = key;
+        const uint32_t u = weight_order(w[e]);
+        if (u < least && t[e] < newest && j + e < p.budget) { least = u; slot = (uint32_t)j + e; }
       }
     };
     for (int64_t j = ((int64_t)rank * NT + tid) * 4; j < p.budget; j += 2 * step) {
@@ -76,6 +79,7 @@ __global__ void __launch_bounds__(NT) paged_evict_kernel(PagedEvictParams p) {
       take(f0, j);
       take(f1, j + step);
     }
+    if (least != 0xffffffffu) best = ((unsigned long long)least << 32) | slot;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
