@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
     }
     const float gj = reinterpret_cast<const float*>(st + OFF_G)[key];
     const float fj = p.f_q ? reinterpret_cast<const float*>(st + OFF_F)[key] : 0.f;
-    const float dec = exp2f(fmin_nan((gq - gj) * kLOG2E, 0.f));
+    const float dec = ex2_approx(fmin_nan((gq - gj) * kLOG2E, 0.f));
     float x = fmaf(reduce_scatter8(qk, part), c1, lam2 * (dec * reduce_scatter8(cb, part)));
     x = (mask >> key) & 1 ? fmaf(fq - fj, kLOG2E, x) : -INFINITY;
     if constexpr (kScores) {
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
       lsum *= corr;
       m_ref = mx;
     }
-    const float pj = exp2f(x - (m_ref == -INFINITY ? 0.f : m_ref));
+    const float pj = ex2_approx(x - (m_ref == -INFINITY ? 0.f : m_ref));   // below 2^-126: 0
     lsum += pj;
     if (mask == 0xffffffffu) {
 #pragma unroll
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
         const int page = page_of(p.pg, (int)b, j, nullptr);
         if (page < 0) continue;
         const int64_t slot = page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
-        p.weight_out[slot] = p.pg.weight[slot] + exp2f(s_x[j] - s_lse);
+        p.weight_out[slot] = p.pg.weight[slot] + ex2_approx(s_x[j] - s_lse);
       }
     }
   }
@@ -598,8 +598,8 @@ __global__ void __launch_bounds__(WT) paged_weights_kernel(PagedAttnParams p) {
       g.x = *reinterpret_cast<const float4*>(xs + j + step);
     }
     if (f.at >= 0) {
-      f.w.x += exp2f(f.x.x - lse); f.w.y += exp2f(f.x.y - lse);
-      f.w.z += exp2f(f.x.z - lse); f.w.w += exp2f(f.x.w - lse);
+      f.w.x += ex2_approx(f.x.x - lse); f.w.y += ex2_approx(f.x.y - lse);
+      f.w.z += ex2_approx(f.x.z - lse); f.w.w += ex2_approx(f.x.w - lse);
       float* out = p.weight_out + f.at;
       if (j + 4 <= n) {
         *reinterpret_cast<float4*>(out) = f.w;
