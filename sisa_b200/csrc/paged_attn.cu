@@ -19,8 +19,8 @@
 // CTA, that paged_join_kernel merges in order (deterministic, no atomics). With weights, the scores are kept
 // in the workspace (4 bytes per key) and paged_weights_kernel adds the shares once lse is known.
 //
-// Measured (B200, a copy moves 6.55 TB/s): 64 sequences of 8192 keys x 16 heads 404 us = 6.80 TB/s, with weights
-// 468 us = 6.03 TB/s; one of 131,071 keys x 16 heads 122 us = 5.6 TB/s, of which about 10 us are start-up and join.
+// Measured (B200, a copy moves 6.55 TB/s): 64 sequences of 8192 keys x 16 heads 403 us = 6.84 TB/s, with weights
+// 461 us = 6.11 TB/s; one of 131,071 keys x 16 heads 120 us = 5.75 TB/s, of which about 10 us are start-up and join.
 // Ten warps per SM with two stages each: four warps with five stages (one CTA per SM) took 504 us on the first
 // case before the waves, since a lone warp per scheduler hides none of its own latency.
 #include <cuda_runtime.h>
