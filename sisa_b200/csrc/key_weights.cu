@@ -30,7 +30,8 @@ namespace sisa {
 namespace kwt {
 
 constexpr int BK = 128, BQ = 64, NSTAGE = 3, NCW = 8;            // keys, queries per tile, stages, compute warps
-constexpr int NG = NCW / 4, NC = BQ / NG, CH = 16;              // warps per key row, query columns of each, columns at a time
+constexpr int NG = NCW / 4, NC = BQ / NG;                        // warps per key row, query columns of each
+constexpr int CH = 16;                                           // columns read at a time
 constexpr uint32_t SZ_K = BK * 128, SZ_B = BK * 64;
 constexpr uint32_t SZ_Q = BQ * 128, SZ_C = BQ * 64, SZ_POS = BQ * 16, SZ_LSE = BQ * 4;
 constexpr uint32_t OFFS_C = SZ_Q, OFFS_POS = OFFS_C + SZ_C, OFFS_LSE = OFFS_POS + SZ_POS;

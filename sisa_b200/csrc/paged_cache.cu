@@ -34,10 +34,11 @@ __device__ __forceinline__ unsigned long long cluster_load(const unsigned long l
 // newest (token < position - recent), the lowest slot where several weigh the same; -1 while the sequence
 // holds fewer than budget keys. (weight, slot) is one 64-bit number, so the minimum does not depend on the
 // order in which it is taken.
-// HBM-bound: 8 bytes per key (64 x 16 units of 8192 slots, 67 MB: 13.5 us; one slot per thread and step: 38 us;
-// 64-bit comparisons per slot: 16.6 us; one or four steps in flight: 14.5 and 20.6 us). A thread takes four slots at a time (16-byte loads of both planes), two such
+// HBM-bound: 8 bytes per key. A thread takes four slots at a time (16-byte loads of both planes), two such
 // steps in flight; a cluster of blocks shares a unit when there are few units, and its first block takes
-// the minimum over the others' through distributed shared memory.
+// the minimum over the others' through distributed shared memory. 64 x 16 units of 8192 slots (67 MB): 13.5 us;
+// one step in flight 14.5 us; with 64-bit comparisons per slot 16.6 us (four steps: 20.6 us); the first version,
+// one slot per thread and step, 38 us.
 constexpr int EVICT_CLUSTER = 8;                 // portable cluster size
 __global__ void __launch_bounds__(NT) paged_evict_kernel(PagedEvictParams p) {
   const int cs = cluster_blocks(), rank = blockIdx.x % cs;

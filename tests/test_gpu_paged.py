@@ -1,10 +1,11 @@
 """The paged-cache operators (sisa_b200/kernels/paged.py) against plain fp64 implementations on the host.
 
 Tolerances, derived from the arithmetic: outputs stored in 16 bits carry one rounding (half an ulp: at most
-2^-8 of the value in bf16 with its 8 significant bits, 2^-11 in fp16 with 11) on an fp32 result, whose own error comes from the exponents. A score in
-log2 units of magnitude up to 2^5 that is summed from about a hundred fp32 products is off by at most about
-100 x 2^-24 x 2^5 = 2e-4 in the worst case and by 1e-5 in practice, so shares and log-sum-exps are held to
-5e-5 (relative to a share, absolute for a log-sum-exp of that magnitude); choices and copies are exact.
+2^-8 of the value in bf16 with its 8 significant bits, 2^-11 in fp16 with 11) on an fp32 result, whose own
+error comes from the exponents. A score in log2 units of magnitude up to 2^5 that is summed from about a
+hundred fp32 products is off by at most about 100 x 2^-24 x 2^5 = 2e-4 in the worst case and by 1e-5 in
+practice, so shares and log-sum-exps are held to 5e-5 (relative to a share, absolute for a log-sum-exp of that
+magnitude); choices and copies are exact.
 """
 from __future__ import annotations
 
