@@ -1,5 +1,7 @@
 // paged_capi.cu - the extern "C" entry points of the paged cache: argument checks and launches. No device
-// allocation, no host synchronisation, no exceptions.
+// allocation, no host synchronisation, no exceptions. Every call makes the device that owns the pages current
+// while it launches: the stream handle 0 names the current device's default stream, and a kernel launched on
+// another GPU would run there with these addresses.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -90,6 +92,8 @@ int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, 
   if (weight_out && !pages->weight) return fail(SISA_ERR_VALUE, what, "weight_out is given but the pages hold no weight");
   if (!aligned(workspace, 16) || !aligned(weight_out, 16))
     return fail(SISA_ERR_ALIGN, what, "workspace and weight_out must be 16-byte aligned");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(pages->k))) return rc;
   p.q = static_cast<const char*>(q->data); p.q_sb = q->stride_b; p.q_sh = q->stride_h;
   p.c = static_cast<const char*>(c->data); p.c_sb = c->stride_b; p.c_sh = c->stride_h;
   p.g_q = g_q; p.f_q = f_q; p.lengths = lengths; p.lam = lam;
@@ -112,6 +116,8 @@ int sisa_paged_evict(const sisa_pages* pages, const int32_t* table, int64_t tabl
   if (budget < 1 || budget > max_pages * pages->page_size)
     return fail(SISA_ERR_VALUE, what, "budget outside [1, max_pages * page_size]");
   if (recent < 0 || recent >= budget) return fail(SISA_ERR_VALUE, what, "recent outside [0, budget)");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(pages->weight))) return rc;
   p.position = position; p.B = (int)B; p.H = (int)H; p.budget = budget; p.recent = recent; p.slots = slots;
   p.status = status;
   return launched(sisa::launch_paged_evict(p, static_cast<cudaStream_t>(stream)), what);
@@ -136,6 +142,8 @@ int sisa_paged_append(const void* proj, int64_t proj_sb, const float* z, int64_t
   if ((rc = sisa_fused_layout(H, off))) return rc;
   if (!aligned(proj, 4) || proj_sb < off[7] || proj_sb % 2 || !aligned(c_out, 4))
     return fail(SISA_ERR_ALIGN, what, "proj rows must hold 273 H elements, 4-byte aligned with an even stride");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(pages->k))) return rc;
   p.proj = static_cast<const uint16_t*>(proj); p.proj_sb = proj_sb; p.z = z; p.z_sb = z_sb;
   p.col_k = (int)off[1]; p.col_v = (int)off[2]; p.col_b = (int)off[3]; p.col_c = (int)off[4];
   p.col_th = (int)off[5]; p.col_a = (int)off[6];
@@ -166,6 +174,8 @@ int sisa_paged_fill(const sisa_pages* pages, const int32_t* table, int64_t table
   if (recent < 0 || recent > keep) return fail(SISA_ERR_VALUE, what, "recent outside [0, keep]");
   if (!weight && keep != L) return fail(SISA_ERR_VALUE, what, "keeping fewer than L keys needs their weights");
   if (!aligned(workspace, 16)) return fail(SISA_ERR_ALIGN, what, "workspace must be 16-byte aligned");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(pages->k))) return rc;
   p.k = static_cast<const char*>(k->data); p.k_sb = k->stride_b; p.k_sh = k->stride_h; p.k_sl = k->stride_l;
   p.v = static_cast<const char*>(v->data); p.v_sb = v->stride_b; p.v_sh = v->stride_h; p.v_sl = v->stride_l;
   p.b = static_cast<const char*>(b->data); p.b_sb = b->stride_b; p.b_sh = b->stride_h; p.b_sl = b->stride_l;
