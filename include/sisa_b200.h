@@ -5,9 +5,9 @@
  * Nothing in this library allocates device memory, synchronises the host or throws across the
  * ABI: the caller owns every output and workspace buffer, and the work is ordered only by the
  * stream that is passed in. Kernels never trap; run-time conditions are OR-ed into *status
- * (SISA_ST_* bits) and left for the caller to read. Entry points that need a current context (to
- * encode TMA tensor maps) make the device that owns their data current for the length of the call
- * and give the calling thread back its previous context before they return.
+ * (SISA_ST_* bits) and left for the caller to read. Every entry point that launches makes the device
+ * that owns its data current for the length of the call and gives the calling thread back its previous
+ * context before it returns (data in host memory is refused); the stream must belong to that device.
  *
  * Reference interfaces (tlstngud/sisa, paths inside that project) that each entry point
  * replaces are cited beside it.

@@ -256,6 +256,8 @@ int sisa_prep_fwd(const void* proj, int64_t B, int64_t L, int64_t H, int64_t pro
     return fail(SISA_ERR_ALIGN, "proj must be 16-byte aligned with strides that are multiples of 8 elements");
   if (!aligned16(c_rot) || !aligned16(b_rot) || !aligned16(pos))
     return fail(SISA_ERR_ALIGN, "c_rot, b_rot and pos must be 16-byte aligned");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(proj))) return rc;
   sisa::PrepFwdLaunch p{};
   p.proj = proj; p.proj_sb = proj_sb; p.proj_sl = proj_sl; p.dtype = dtype;
   p.z = z; p.z_sb = z_sb; p.z_sl = z_sl;
@@ -274,6 +276,8 @@ int sisa_pack_positions(const float* g, int64_t g_sb, int64_t g_sh, int64_t g_sl
   if ((rc = check_dims(B, H, L))) return rc;
   if (!g || !pos) return fail(SISA_ERR_VALUE, "sisa_pack_positions: null pointer");
   if (!aligned16(pos)) return fail(SISA_ERR_ALIGN, "pos must be 16-byte aligned");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(g))) return rc;
   sisa::PackLaunch p{};
   p.g = g; p.g_sb = g_sb; p.g_sh = g_sh; p.g_sl = g_sl;
   p.f = fgate; p.f_sb = f_sb; p.f_sh = f_sh; p.f_sl = f_sl;
@@ -438,6 +442,8 @@ int sisa_prep_bwd(const void* proj, int64_t B, int64_t L, int64_t H, int64_t pro
     return fail(SISA_ERR_ALIGN, "proj/dproj must be 16-byte aligned with strides that are multiples of 8");
   if (!aligned16(dc) || !aligned16(db) || !aligned16(workspace))
     return fail(SISA_ERR_ALIGN, "dc, db and workspace must be 16-byte aligned");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(proj))) return rc;
   sisa::PrepBwdLaunch p{};
   p.proj = proj; p.proj_sb = proj_sb; p.proj_sl = proj_sl; p.dtype = dtype;
   p.z = z; p.z_sb = z_sb; p.z_sl = z_sl;
@@ -471,6 +477,8 @@ static int decode_attn_impl(const sisa_view4* q, const sisa_view4* c, const floa
     return fail(SISA_ERR_VALUE, "sisa_decode_attn: f_q and f_cache must both be given or both be null");
   if (gf_stride < N) return fail(SISA_ERR_VALUE, "g/F cache row stride %lld < N %lld", (long long)gf_stride,
                                  (long long)N);
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(q->data))) return rc;
   sisa::DecodeParams p{};
   p.q = static_cast<const char*>(q->data); p.q_sb = q->stride_b; p.q_sh = q->stride_h;
   p.c = static_cast<const char*>(c->data); p.c_sb = c->stride_b; p.c_sh = c->stride_h;
@@ -539,6 +547,8 @@ static int decode_prep_impl(const void* proj, int64_t proj_sb, const float* z, i
       (v_cache->stride_b | v_cache->stride_h | v_cache->stride_l) % 2 ||
       (b_cache->stride_b | b_cache->stride_h | b_cache->stride_l) % 2)
     return fail(SISA_ERR_ALIGN, "sisa_decode_prep: operands need 4-byte alignment and even element strides");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(proj))) return rc;
   sisa::DecodePrepParams p{};
   p.proj = static_cast<const uint16_t*>(proj); p.proj_sb = proj_sb;
   p.z = z; p.z_sb = z_sb;
@@ -658,6 +668,8 @@ int sisa_lce_grad(void* logits, int64_t logits_ld, int64_t R, int64_t V, int64_t
   if (!logits || !labels || !inv_n || !workspace || !loss_rows) return fail(SISA_ERR_VALUE, "sisa_lce_grad: null pointer");
   if (R < 1 || Vp % 128 || Vp < V || logits_ld < Vp || logits_ld % 8 || !aligned16(logits))
     return fail(SISA_ERR_VALUE, "sisa_lce_grad: bad shape or alignment");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(logits))) return rc;
   const int64_t nseg = (Vp + 255) / 256;
   sisa::LceGradParams p{};
   p.logits = static_cast<char*>(logits); p.ld = logits_ld;
@@ -1050,6 +1062,8 @@ int sisa_norm_fwd(const sisa_norm_fwd_args* a, int32_t* status, void* stream) {
   if (a->xsum && !a->res) return fail(SISA_ERR_VALUE, "sisa_norm_fwd: xsum without res");
   if (a->n_proj > 0 && (!a->proj_w || !a->proj_b || !a->proj_out))
     return fail(SISA_ERR_VALUE, "sisa_norm_fwd: n_proj > 0 needs proj_w, proj_b and proj_out");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(a->x))) return rc;
   sisa::NormFwd p{};
   p.x = a->x; p.xs = a->x_ld; p.xdt = a->x_dtype;
   p.res = a->res; p.ress = a->res_ld; p.resdt = a->res ? a->res_dtype : 2;
@@ -1087,6 +1101,8 @@ int sisa_norm_bwd(const sisa_norm_bwd_args* a, int32_t* status, void* stream) {
     return fail(SISA_ERR_VALUE, "sisa_norm_bwd: weight gradients need the workspace");
   if (a->n_proj == 0 && (a->dproj_w || a->dproj_b))
     return fail(SISA_ERR_VALUE, "sisa_norm_bwd: dproj_w / dproj_b without a projection");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(a->v))) return rc;
   sisa::NormBwd p{};
   p.v = a->v; p.vs = a->v_ld; p.vdt = a->v_dtype;
   p.w = a->weight; p.rstd = a->rstd; p.rows = a->rows; p.d = a->d;
@@ -1135,6 +1151,8 @@ int sisa_swiglu_fwd(const void* g, int64_t g_ld, const void* u, int64_t u_ld, in
   int rc;
   if ((rc = check_swiglu(rows, f, dtype, "sisa_swiglu_fwd"))) return rc;
   if (!g || !u || !a || g_ld < f || u_ld < f || a_ld < f) return fail(SISA_ERR_VALUE, "sisa_swiglu_fwd: null pointer or stride");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(g))) return rc;
   sisa::SwiGluFwd p{g, g_ld, u, u_ld, rows, f, a, a_ld, dtype};
   cudaError_t e = sisa::launch_swiglu_fwd(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? SISA_OK : cuda_fail(e, "sisa_swiglu_fwd launch");
@@ -1148,6 +1166,8 @@ int sisa_swiglu_bwd(const void* da, int64_t da_ld, const void* g, int64_t g_ld, 
   if ((rc = check_swiglu(rows, f, dtype, "sisa_swiglu_bwd"))) return rc;
   if (!da || !g || !u || !dg || !du || da_ld < f || g_ld < f || u_ld < f || dg_ld < f || du_ld < f)
     return fail(SISA_ERR_VALUE, "sisa_swiglu_bwd: null pointer or stride");
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(g))) return rc;
   sisa::SwiGluBwd p{da, da_ld, g, g_ld, u, u_ld, rows, f, dg, dg_ld, du, du_ld, dtype};
   cudaError_t e = sisa::launch_swiglu_bwd(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? SISA_OK : cuda_fail(e, "sisa_swiglu_bwd launch");

@@ -64,6 +64,9 @@ extern "C" int sisa_selftest_wait(int producer_arrives, int64_t limit_ns, int32_
   if (limit_ns < 1000 || limit_ns > 1000000000)
     return sisa::capi_fail(SISA_ERR_VALUE, "sisa_selftest_wait: limit_ns must lie in [1e3, 1e9]");
   if (!result) return sisa::capi_fail(SISA_ERR_VALUE, "sisa_selftest_wait: null result");
+  int rc;
+  sisa::DeviceScope scope;
+  if ((rc = scope.bind(result))) return rc;
   sisa::selftest::wait_kernel<<<1, 128, 0, static_cast<cudaStream_t>(stream)>>>(
       producer_arrives, (uint64_t)limit_ns, status, result);
   return cudaGetLastError() == cudaSuccess ? SISA_OK

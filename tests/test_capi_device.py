@@ -40,6 +40,36 @@ def paged_calls(lib):
     }
 
 
+def other_calls(lib):
+    k, b = view(64), view(32)
+    nf, nb = _lib.NormFwdArgs(), _lib.NormBwdArgs()
+    for a in (nf, nb):
+        for name, value in (("weight", A), ("rstd", A), ("rows", 4), ("d", 64)):
+            setattr(a, name, value)
+    nf.x, nf.x_ld, nf.x_dtype, nf.n_out, nf.eps = A, 64, BF16, 1, 1e-6
+    nf.y[0], nf.y_ld[0], nf.y_dtype[0] = A, 64, BF16
+    nb.v, nb.v_ld, nb.v_dtype, nb.dx, nb.dx_ld, nb.dx_dtype = A, 64, BF16, A, 64, BF16
+    nb.dy[0], nb.dy_ld[0], nb.dy_dtype[0] = A, 64, BF16
+    attn = (k, b, A, A, k, k, b, A, A, 200, A, 3, 2)
+    prep = (A, 560, A, 2, 3, 2, BF16, k, k, b, A, A, 200)
+    return {
+        "sisa_prep_fwd": lambda: lib.sisa_prep_fwd(A, 3, 200, 2, 560 * 200, 560, BF16, A, 400, 2, A, A, A, A, None, None),
+        "sisa_pack_positions": lambda: lib.sisa_pack_positions(A, 400, 200, 1, A, 400, 200, 1, 3, 2, 200, A, None, None),
+        "sisa_prep_bwd": lambda: lib.sisa_prep_bwd(A, 3, 200, 2, 560 * 200, 560, BF16, A, 400, 2, A, A, A, A, A, A, 560 * 200, 560,
+                                                   A, A, None, None),
+        "sisa_decode_attn": lambda: lib.sisa_decode_attn(*attn, 200, BF16, k, A, None, None),
+        "sisa_decode_attn_dpos": lambda: lib.sisa_decode_attn_dpos(*attn, A, 200, BF16, k, A, None, None),
+        "sisa_decode_prep": lambda: lib.sisa_decode_prep(*prep, 7, A, A, A, A, None, None),
+        "sisa_decode_prep_dpos": lambda: lib.sisa_decode_prep_dpos(*prep, A, 100, A, A, A, A, None, None),
+        "sisa_lce_grad": lambda: lib.sisa_lce_grad(A, 128, 4, 100, 128, BF16, A, -100, A, 1.0, 1, A, A, None, None),
+        "sisa_norm_fwd": lambda: lib.sisa_norm_fwd(_lib.vref(nf), None, None),
+        "sisa_norm_bwd": lambda: lib.sisa_norm_bwd(_lib.vref(nb), None, None),
+        "sisa_swiglu_fwd": lambda: lib.sisa_swiglu_fwd(A, 64, A, 64, 4, 64, BF16, A, 64, None, None),
+        "sisa_swiglu_bwd": lambda: lib.sisa_swiglu_bwd(A, 64, A, 64, A, 64, 4, 64, BF16, A, 64, A, 64, None, None),
+        "sisa_selftest_wait": lambda: lib.sisa_selftest_wait(1, 1000000, None, A, None),
+    }
+
+
 def ends_at_the_look_up(call):
     rc = call()
     message = _lib.last_error()
@@ -50,4 +80,12 @@ def ends_at_the_look_up(call):
                                   "sisa_attn_key_weights"])
 def test_paged_calls_bind_the_device_of_their_pages(name):
     ok, got = ends_at_the_look_up(paged_calls(_lib.load())[name])
+    assert ok, got
+
+
+@pytest.mark.parametrize("name", ["sisa_prep_fwd", "sisa_pack_positions", "sisa_prep_bwd", "sisa_decode_attn",
+                                  "sisa_decode_attn_dpos", "sisa_decode_prep", "sisa_decode_prep_dpos", "sisa_lce_grad",
+                                  "sisa_norm_fwd", "sisa_norm_bwd", "sisa_swiglu_fwd", "sisa_swiglu_bwd", "sisa_selftest_wait"])
+def test_the_other_calls_bind_the_device_of_their_data(name):
+    ok, got = ends_at_the_look_up(other_calls(_lib.load())[name])
     assert ok, got
