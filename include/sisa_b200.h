@@ -26,7 +26,8 @@ extern "C" {
 #define SISA_ST_NONMONOTONE 2  /* g rose by more than 1e-3 between neighbours (attention.py:123-125,675-683) */
 #define SISA_ST_TIMEOUT     4  /* a bounded device wait gave up; results are invalid */
 #define SISA_ST_BAD_SEED    8  /* linear-CE backward seed differs from the promised grad_scale (linear_ce.py:202-206) */
-#define SISA_ST_BAD_POS    16  /* a decode position read on the device lay outside the cache; nothing was written */
+#define SISA_ST_BAD_POS    16  /* a position, length, slot or page read on the device lay outside the cache; nothing was
+                                * written there */
 
 /* ---- return codes ---- */
 #define SISA_OK              0
@@ -386,8 +387,8 @@ typedef struct sisa_pages {
  * lengths (B,) int32; y (B, H, 1, 64) view; lse (B, H) fp32 in log2 units, or NULL. With weight_out (a plane
  * with the strides of pages->weight, which it may be) every key's share is added:
  * weight_out_j = weight_j + softmax(s)_j; slots past a sequence's length are not written. A sequence of
- * length <= 0 gives y = 0 and lse = -inf; a length above max_pages * page_size is cut there and sets
- * SISA_ST_BAD_POS. workspace: sisa_paged_attn_workspace(B, H, max_pages * page_size, weight_out != NULL)
+ * length <= 0, or one whose keys are all left out, gives y = 0 and lse = -inf; a length above max_pages * page_size
+ * is cut there and sets SISA_ST_BAD_POS. workspace: sisa_paged_attn_workspace(B, H, max_pages * page_size, weight_out != NULL)
  * bytes, 16-byte aligned, one call at a time (NULL where that is 0: short tables). Deterministic. */
 int64_t sisa_paged_attn_workspace(int64_t B, int64_t H, int64_t max_keys, int accumulate);
 int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, const float* f_q,

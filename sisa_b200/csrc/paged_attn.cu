@@ -3,7 +3,8 @@
 // For every sequence b with n_b keys (slots 0 .. n_b - 1 of its pages, in any order) and head h:
 //   x_j = log2e (q.k_j / 8 + lam_h exp(min(g_q - g_j, 0)) (c.b~_j) + (F_q - F_j)),
 //   y = sum_j 2^(x_j - lse) v_j,  lse = log2 sum_j 2^x_j,  and optionally weight_j += 2^(x_j - lse).
-// A row with no keys gives y = 0 and lse = -inf.
+// A row with no keys, or whose keys are all left out (table entries that name no page) or all score -inf,
+// gives y = 0, lse = -inf and no shares.
 //
 // HBM-bound: 328 bytes per key and head (k, v, b~ in 16 bits, g and F in 32), 320 flops. Work is cut into
 // tiles of 32 keys; the tiles of all (sequence, head) units lie in one line, and each of a fixed number of
@@ -175,19 +176,37 @@ struct Sum {
   }
 };
 
+// The log-sum-exp of a unit of sequence b from its maximum and sum, the same in all lanes of the warp, and r = 1 / l
+// (0 where no key has a share). A value that is not finite sets SISA_ST_NONFINITE, except where no key lies in a
+// page of the pool: those table entries have set SISA_ST_BAD_POS, and nothing was read that could be at fault.
+__device__ __forceinline__ float row_lse(const PagedAttnParams& p, int b, float m, float l, float& r) {
+  const float lse = m + log2f(l);
+  r = l == 0.f ? 0.f : 1.f / l;
+  if (!isfinite(lse)) {
+    const int lane = threadIdx.x & 31;
+    bool any = l != 0.f;
+    const int64_t pages = (keys_of(p, b) + (int64_t(1) << p.pg.page_shift) - 1) >> p.pg.page_shift;
+    for (int64_t i = lane; i < pages && !any; i += 32)
+      any = (unsigned)__ldg(p.pg.table + (int64_t)b * p.pg.table_sb + i) < (unsigned)p.pg.n_pages;
+    if (__any_sync(0xffffffffu, any) && lane == 0 && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
+  }
+  return lse;
+}
+
 // y and lse of unit bh = (b, h) from its complete sum.
 template <bool kHalf>
 __device__ __forceinline__ float write_row(const PagedAttnParams& p, int64_t bh, const Sum& s) {
   const int64_t b = bh / p.H, h = bh % p.H;
   const int lane = threadIdx.x & 31;
-  const float lse = s.m + log2f(s.l), r = 1.f / s.l;
+  float r;
+  const float lse = row_lse(p, (int)b, s.m, s.l, r);
   reinterpret_cast<uint32_t*>(p.y + 2 * (b * p.y_sb + h * p.y_sh))[lane] = pack2<kHalf>(s.a.x * r, s.a.y * r);
-  if (lane == 0) {
-    if (p.lse_all) p.lse_all[bh] = lse;
-    if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
-  }
+  if (lane == 0 && p.lse_all) p.lse_all[bh] = lse;
   return lse;
 }
+
+// What a share's exponent is relative to: lse, or 0 where every score is -inf and no key has a share.
+__device__ __forceinline__ float share_base(float lse) { return lse == -INFINITY ? 0.f : lse; }
 
 // kUnit: a CTA has one unit to itself, its warps equal runs of that unit's tiles; y, lse and (from the scores
 // kept in shared memory) the weights are finished here and no other kernel follows.
@@ -398,7 +417,8 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
       for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
       const int64_t bh = (int64_t)at.b * p.H + at.h;
       if (seg == at.T) {                        // the whole unit
-        const float lse = m_ref + log2f(lsum), r = 1.f / lsum;
+        float r;
+        const float lse = row_lse(p, at.b, m_ref, lsum, r);
         if (quad == 0) {
           const uint4 o = make_uint4(pack2<kHalf>(acc[0].x * r, acc[0].y * r), pack2<kHalf>(acc[1].x * r, acc[1].y * r),
                                      pack2<kHalf>(acc[2].x * r, acc[2].y * r), pack2<kHalf>(acc[3].x * r, acc[3].y * r));
@@ -407,7 +427,6 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
         if (lane == 0) {
           if (kUnit) s_lse = lse;
           if (!kUnit || p.lse_all) p.lse_all[bh] = lse;
-          if (!isfinite(lse) && p.status) atomicOr(p.status, SISA_ST_NONFINITE);
         }
       } else {
         const int kind = at.t + 1 == seg ? 1 : 0;
@@ -471,11 +490,12 @@ __global__ void __launch_bounds__(NW * 32, 2) paged_attn_kernel(PagedAttnParams 
     }
     if constexpr (kScores) {
       __syncthreads();
+      const float lse = share_base(s_lse);
       for (int64_t j = threadIdx.x; j < n; j += NW * 32) {
         const int page = page_of(p.pg, (int)b, j, nullptr);
         if (page < 0) continue;
         const int64_t slot = page * p.pg.s_sp + h * p.pg.s_sh + (j & ((1 << p.pg.page_shift) - 1));
-        p.weight_out[slot] = p.pg.weight[slot] + ex2_approx(s_x[j] - s_lse);
+        p.weight_out[slot] = p.pg.weight[slot] + ex2_approx(s_x[j] - lse);
       }
     }
   }
@@ -589,7 +609,7 @@ __global__ void __launch_bounds__(WT) paged_weights_kernel(PagedAttnParams p) {
     if (threadIdx.x == 0 && n > 0) s_lse = joined ? sum.m + log2f(sum.l) : p.lse_all[bh];
   }
   __syncthreads();
-  const float lse = s_lse;
+  const float lse = share_base(s_lse);
   for (; j - threadIdx.x * 4 < n; j += step) {
     Four g;
     g.at = place(j + step);
