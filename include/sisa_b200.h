@@ -368,7 +368,10 @@ int sisa_decode_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q,
  * 128 or 256. f may be NULL without a forget gate; weight and token where nothing is evicted.
  * table: (B, max_pages) int32, row stride table_sb: the page of each block of page_size slots of a
  * sequence. Entries are read only where a slot is used; one outside [0, n_pages) sets SISA_ST_BAD_POS and
- * its keys are left out. B*H <= 65,535. */
+ * its keys are left out. Rows may name the same page (a shared prefix) where a call only reads it. A page that a
+ * call writes, and with accumulated weights a page that it reads, belongs to one entry of the table: the calls
+ * add and store without atomics, so a second row's shares or keys would be lost in part, differently from run to
+ * run. B*H <= 65,535. */
 typedef struct sisa_pages {
   void* k;
   void* v;
@@ -389,7 +392,8 @@ typedef struct sisa_pages {
  * weight_out_j = weight_j + softmax(s)_j; slots past a sequence's length are not written. A sequence of
  * length <= 0, or one whose keys are all left out, gives y = 0 and lse = -inf; a length above max_pages * page_size
  * is cut there and sets SISA_ST_BAD_POS. workspace: sisa_paged_attn_workspace(B, H, max_pages * page_size, weight_out != NULL)
- * bytes, 16-byte aligned, one call at a time (NULL where that is 0: short tables). Deterministic. */
+ * bytes, 16-byte aligned, one call at a time (NULL where that is 0: short tables). Deterministic (with weight_out,
+ * as long as no page of a used slot is named twice in the table). */
 int64_t sisa_paged_attn_workspace(int64_t B, int64_t H, int64_t max_keys, int accumulate);
 int sisa_paged_attn(const sisa_view4* q, const sisa_view4* c, const float* g_q, const float* f_q,
                     const sisa_pages* pages, const int32_t* table, int64_t table_sb, int64_t max_pages,

@@ -12,6 +12,9 @@ the slots may hold the keys in any order.
 All functions run on torch's current stream and follow the check mode of :mod:`sisa_b200.backends`;
 ``block_table`` is (B, max_pages) int32, ``lengths`` and ``position`` are (B,) int32 on the device, so
 that a captured CUDA graph serves every step.
+
+Rows of a block table may share pages (a common prefix) only in calls that read them: :func:`paged_attention`
+without ``accumulate``. A page that a call writes, or whose weights it adds to, has to belong to one row.
 """
 from __future__ import annotations
 
@@ -140,7 +143,8 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
     ``return_lse``, (y, lse) with lse (B, H) fp32 in log2 units (-inf for an idle row).
 
     With ``accumulate`` each key's softmax share is added to its weight: ``pages.weight`` in place, or
-    ``weight_out`` = ``pages.weight`` + share where that plane is given (used slots only)."""
+    ``weight_out`` = ``pages.weight`` + share where that plane is given (used slots only). No two rows may then
+    share a page: both would add to the same weights, and one of the shares could be lost."""
     B, H = _check_query(q, c, pages)
     lib = _lib.load()
     dev = pages.device

@@ -89,3 +89,25 @@ def test_a_row_whose_scores_are_all_minus_infinity(cuda_dev, n, wide):
         backends.check_status(cuda_dev)
     assert bool((y == 0).all()) and bool((lse == -math.inf).all())
     assert torch.equal(get(pages.weight, table, 0, n), rows[0]["w"])
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_rows_may_share_the_pages_they_read(cuda_dev, wide):
+    """Four queries over a common prefix of three pages, each with an own page after it."""
+    from sisa_b200 import backends
+
+    S, H, lengths = 32, 3, [100, 128, 97, 121]
+    pages, table, rows, x = attn_case([128] * 4, H, S, torch.bfloat16, cuda_dev, seed=8)
+    shared = table.clone()
+    shared[1:, :3] = table[0, :3]
+    for i, n in enumerate(lengths):
+        for name in ("k", "v", "b", "g", "f", "w"):
+            rows[i][name] = torch.cat([rows[0][name][:, :96], rows[i][name][:, 96:n]], dim=1)
+    before = pages.weight.clone()
+    y, lse = call(pages, widen(shared) if wide else shared, lengths, x, cuda_dev)
+    backends.check_status(cuda_dev)
+    for i, (yr, lr, _) in enumerate(attn_truth(rows, lengths, x)):
+        bound = HALF_ULP[y.dtype] * yr.abs() * (1 + 1e-3) + SHARE_REL * rows[i]["v"].abs().max()
+        assert bool(((y[i, :, 0].double().cpu() - yr).abs() <= bound).all())
+        assert max_abs(lse[i], lr) <= 5e-5 * max(1.0, float(lr.abs().max()) / 32)
+    assert torch.equal(pages.weight.nan_to_num(-1.0), before.nan_to_num(-1.0))
