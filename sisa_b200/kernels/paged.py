@@ -11,7 +11,8 @@ the slots may hold the keys in any order.
 
 All functions run on torch's current stream and follow the check mode of :mod:`sisa_b200.backends`;
 ``block_table`` is (B, max_pages) int32, ``lengths`` and ``position`` are (B,) int32 on the device, so
-that a captured CUDA graph serves every step.
+that a captured CUDA graph serves every step. They are for serving and have no backward: an input that
+requires a gradient, in grad mode, raises ValueError.
 
 Rows of a block table may share pages (a common prefix) only in calls that read them: :func:`paged_attention`
 without ``accumulate``. A page that a call writes, or whose weights it adds to, has to belong to one row.
@@ -63,6 +64,7 @@ class KeyPages:
                 raise TypeError(f"plane {name} must be {dt}, got {t.dtype}")
         if any(t is not None and t.device != k.device for t in (v, b, g, f, weight, token)):
             raise ValueError("all pages must lie on one device")
+        _refuse_grad("KeyPages", k, v, b, g, f, weight)
         self.k, self.v, self.b, self.g, self.f, self.weight, self.token = k, v, b, g, f, weight, token
         self.n_pages, self.n_head, self.page_size = P, H, S
         self.dtype, self.device = k.dtype, k.device
@@ -84,6 +86,15 @@ class KeyPages:
         weight = torch.empty_like(g) if evict else None
         token = torch.empty(shape, dtype=torch.int32, device=device) if evict else None
         return cls(k, v, b, g, f, weight, token)
+
+
+def _refuse_grad(what: str, *tensors: Tensor | None) -> None:
+    """These operators serve; none has a backward. Where a gradient would be recorded for an input, raise rather than
+    return a result that has lost it."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no backward: call it under torch.no_grad() or with detached inputs")
 
 
 def _table(pages: KeyPages, table: Tensor, B: int) -> tuple[int, int, int]:
@@ -146,6 +157,7 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
     ``weight_out`` = ``pages.weight`` + share where that plane is given (used slots only). No two rows may then
     share a page: both would add to the same weights, and one of the shares could be lost."""
     B, H = _check_query(q, c, pages)
+    _refuse_grad("paged_attention", q, c, g, fgate, lam, weight_out)
     lib = _lib.load()
     dev = pages.device
     tp, tsb, mp = _table(pages, block_table, B)
@@ -227,6 +239,7 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
         raise TypeError(f"projection dtype {proj.dtype} differs from the pages' {pages.dtype}")
     if proj.device != dev:
         raise ValueError(f"proj is on {proj.device}, the pages on {dev}")
+    _refuse_grad("paged_append", proj, z, carry, carry_out)
     tp, tsb, mp = _table(pages, block_table, B)
     pp = _rows(position, (B,), "position", pages)
     sp = None if slots is None else _rows(slots, (B, H), "slots", pages)
@@ -278,6 +291,7 @@ def attention_key_weights(q: Tensor, k: Tensor, c: Tensor, b: Tensor, pos: Tenso
                          f"{tuple(k.shape)}, {tuple(c.shape)} and {tuple(b.shape)}")
     if any(t.dtype != q.dtype for t in (k, c, b)):
         raise TypeError(f"q, k, c and b differ in dtype: {q.dtype}, {k.dtype}, {c.dtype}, {b.dtype}")
+    _refuse_grad("attention_key_weights", q, k, c, b, pos, lam, lse)
     lib = _lib.load()
     code = _lib.dtype_code(q.dtype)
     if pos.shape != (B, H, 4, lib.sisa_pos_len(L)) or not pos.is_contiguous() or pos.dtype != torch.float32:
@@ -315,6 +329,7 @@ def paged_fill(pages: KeyPages, block_table: Tensor, k: Tensor, v: Tensor, b: Te
                          f"{tuple(v.shape)} and {tuple(b.shape)}")
     if k.dtype != pages.dtype or v.dtype != pages.dtype or b.dtype != pages.dtype:
         raise TypeError(f"k, v and b must be {pages.dtype} like the pages, got {k.dtype}, {v.dtype}, {b.dtype}")
+    _refuse_grad("paged_fill", k, v, b, g, fgate, weight)
     dev = pages.device
     for t in (k, v, b, g, fgate, weight):
         if t is not None and t.device != dev:

@@ -111,3 +111,31 @@ def test_rows_may_share_the_pages_they_read(cuda_dev, wide):
         assert bool(((y[i, :, 0].double().cpu() - yr).abs() <= bound).all())
         assert max_abs(lse[i], lr) <= 5e-5 * max(1.0, float(lr.abs().max()) / 32)
     assert torch.equal(pages.weight.nan_to_num(-1.0), before.nan_to_num(-1.0))
+
+
+def test_inputs_that_require_a_gradient_are_refused(cuda_dev):
+    """None of the operators has a backward: in grad mode they raise, under no_grad they run as ever."""
+    from sisa_b200.kernels import paged as K
+    from tests.test_gpu_paged import prompt
+
+    dev, bf = cuda_dev, torch.bfloat16
+    pages, table, rows, x = attn_case([40], 2, 16, bf, dev, seed=1)
+    d = {n: t.to(dev) for n, t in x.items()}
+    ln, pos = (torch.tensor([n], dtype=torch.int32, device=dev) for n in (40, 3))
+    proj, z, carry = torch.zeros(1, 1, 560, dtype=bf, device=dev), torch.zeros(1, 1, 2, device=dev), torch.zeros(1, 2, 18, device=dev)
+    q, k, v, c, b, pl, lam, lse = prompt(1, 2, 40, bf, dev, seed=2)
+    g, f, w = pl[:, :, 0, :40].contiguous(), pl[:, :, 1, :40].contiguous(), torch.rand(1, 2, 40, device=dev)
+    calls = [(lambda *a: K.paged_attention(*a[:4], pages, table, ln, a[4]), [d["q"], d["c"], d["gq"], d["fq"], d["lam"]]),
+             (lambda *a: K.paged_append(a[0], a[1], pages, table, pos, a[2]), [proj, z, carry]),
+             (K.attention_key_weights, [q, k, c, b, pl, lam, lse]),
+             (lambda *a: K.paged_fill(pages, table, *a[:5], weight=a[5]), [k, v, b, g, f, w]),
+             (K.KeyPages, [pages.k, pages.v, pages.b, pages.g, pages.f, pages.weight])]
+    for fn, args in calls:
+        fn(*args)
+        for i in range(len(args)):
+            a = list(args)
+            a[i] = a[i].detach().clone().requires_grad_(True)
+            with pytest.raises(ValueError, match="no backward"):
+                fn(*a)
+            with torch.no_grad():
+                fn(*a)
