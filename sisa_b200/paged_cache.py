@@ -67,11 +67,17 @@ class PagedRows:
     paged = True
 
     def __init__(self, cache: "PagedCache", first: int, count: int):
-        self.cache, self.first, self.count = cache, first, count
+        # the whole cache does not refer to itself: a cycle would keep its pages allocated until the garbage collector runs
+        self._cache = None if cache is self else cache
+        self.first, self.count = first, count
         span = slice(first, first + count)
         self.table, self.position, self.lengths = cache.table[span], cache.position[span], cache.lengths[span]
         self._live = cache.live[span]
         self._range = range(first, first + count)
+
+    @property
+    def cache(self) -> "PagedCache":
+        return self if self._cache is None else self._cache
 
     def carry(self, layer_idx: int) -> Tensor:
         return self.cache.carries[layer_idx, self.first:self.first + self.count]
