@@ -328,7 +328,8 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
     :class:`~sisa_b200.paged_cache.PagedCache` (cuda path only). ``cache_budget`` bounds the keys kept per
     head and sequence: of the prompt the ``cache_recent`` newest (default a quarter) and those that received
     most attention from its last ``cache_observe`` queries (default all), then every new token replaces the
-    least attended old key. Without a budget, or with one that is never reached, nothing is dropped.
+    least attended old key. Without a budget, or with one that the prompt and the new tokens never reach, nothing
+    is dropped and the cache takes pages for these tokens only.
     """
     _check_generate_args(input_ids, max_new_tokens, do_sample, temperature, top_k)
     squeeze = input_ids.dim() == 1
@@ -362,11 +363,14 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
 def _paged_cache(model, input_ids, total, page_size, budget, recent, observe):
     """The paged cache of :func:`generate` (raises where the cuda path cannot run)."""
     from .modeling import _compute_dtype, _resolve_impl
-    from .paged_cache import PagedCache
+    from .paged_cache import PagedCache, resolve_recent
 
     probe = model.embed.weight[:1].detach().unsqueeze(0)
     if not probe.is_cuda or _resolve_impl(model.config.attn_impl, probe, model.config) != "cuda":
         raise ValueError("page_size and cache_budget need the model on the cuda attention path")
+    if budget is not None and budget >= total:   # never reached: pages for the text, not for the budget, and no weights
+        resolve_recent(budget, recent, observe)
+        budget = recent = observe = None
     return PagedCache(model.config, input_ids.shape[0], max_tokens=total if budget is None else None, budget=budget,
                       recent=recent, observe=observe, page_size=64 if page_size is None else page_size,
                       dtype=_compute_dtype(probe), device=probe.device)

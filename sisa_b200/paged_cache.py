@@ -29,6 +29,19 @@ if TYPE_CHECKING:  # pragma: no cover
 __all__ = ["PagedCache", "PagedRows", "PagedLayer"]
 
 
+def resolve_recent(budget: int, recent: int | None, observe: int | None) -> int:
+    """The number of newest keys that are never evicted, by default a quarter of the budget, with the eviction's
+    arguments checked."""
+    if budget < 1:
+        raise ValueError(f"budget must be >= 1, got {budget}")
+    recent = budget // 4 if recent is None else recent
+    if not 0 <= recent < budget:
+        raise ValueError(f"recent must lie in [0, budget), got {recent} with a budget of {budget}")
+    if observe is not None and observe < 1:
+        raise ValueError(f"observe must be >= 1, got {observe}")
+    return recent
+
+
 class PagedLayer:
     """One layer of some rows of a :class:`PagedCache`, as the attention's decode step uses it."""
 
@@ -203,15 +216,11 @@ class PagedCache(PagedRows):
         if page_size not in K.PAGE_SIZES:
             raise ValueError(f"page_size must be one of {K.PAGE_SIZES}, got {page_size}")
         capacity = max_tokens if budget is None else budget
-        if capacity < 1:
-            raise ValueError(f"{'max_tokens' if budget is None else 'budget'} must be >= 1, got {capacity}")
+        if budget is None and max_tokens < 1:
+            raise ValueError(f"max_tokens must be >= 1, got {max_tokens}")
         if budget is None and (recent is not None or observe is not None):
             raise ValueError("recent and observe need a budget")
-        recent = 0 if budget is None else (budget // 4 if recent is None else recent)
-        if budget is not None and not 0 <= recent < budget:
-            raise ValueError(f"recent must lie in [0, budget), got {recent} with a budget of {budget}")
-        if observe is not None and observe < 1:
-            raise ValueError(f"observe must be >= 1, got {observe}")
+        recent = 0 if budget is None else resolve_recent(budget, recent, observe)
         if config.d_head != 64 or config.d_state != 32:
             raise ValueError("the paged cache needs d_head 64 and d_state 32")
         if dtype not in (torch.bfloat16, torch.float16):

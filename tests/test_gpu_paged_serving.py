@@ -58,3 +58,31 @@ def test_generate_leaves_no_cache_behind(cuda_dev, monkeypatch, cuda_graph):
         assert len(made) == 2 and all(r() is None for r in made)
     finally:
         gc.enable()
+
+
+def test_a_budget_beyond_the_text_takes_pages_for_the_text(cuda_dev, monkeypatch):
+    """A budget that the prompt and the new tokens never reach: the pool has the size of the text, the tokens are
+    those without a budget, and the arguments are checked against the budget that was given."""
+    from sisa_b200 import paged_cache
+
+    made = []
+
+    class Recorded(paged_cache.PagedCache):
+        def __init__(self, *a, **kw):
+            super().__init__(*a, **kw)
+            made.append((self.capacity, self.pages[0].n_pages, self.table.shape[1]))
+
+    model = tiny(cuda_dev)
+    ids = ids_of((3, 40), 2, cuda_dev)
+    want = model.generate(ids, max_new_tokens=24, page_size=16)
+    monkeypatch.setattr(paged_cache, "PagedCache", Recorded)
+    for kw in (dict(cache_budget=64), dict(cache_budget=100_000), dict(cache_budget=100_000, cache_recent=70, cache_observe=8)):
+        assert torch.equal(model.generate(ids, max_new_tokens=24, page_size=16, **kw), want)
+    assert made == [(64, 3 * 4, 4)] * 3
+    made.clear()
+    assert model.generate(ids, max_new_tokens=24, page_size=16, cache_budget=63).shape == (3, 64)
+    assert made == [(63, 3 * 4, 4)]
+    for kw in (dict(cache_budget=1000, cache_recent=1000), dict(cache_budget=1000, cache_recent=-1), dict(cache_budget=1000, cache_observe=0),
+               dict(cache_budget=0), dict(page_size=16, cache_recent=2)):
+        with pytest.raises(ValueError):
+            model.generate(ids, max_new_tokens=24, **kw)
