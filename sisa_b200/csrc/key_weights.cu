@@ -243,14 +243,10 @@ __global__ void __launch_bounds__(NT, 3) key_weights_kernel(const __grid_constan
 
 cudaError_t launch_key_weights(const KeyWeightParams& p, int dtype, cudaStream_t st) {
   using namespace kwt;
-  dim3 grid(p.ntk, p.B * p.H);
-  if (dtype == 1) {
-    cudaFuncSetAttribute(key_weights_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    key_weights_kernel<true><<<grid, NT, SMEM_BYTES, st>>>(p);
-  } else {
-    cudaFuncSetAttribute(key_weights_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    key_weights_kernel<false><<<grid, NT, SMEM_BYTES, st>>>(p);
-  }
+  auto* kernel = dtype == 1 ? key_weights_kernel<true> : key_weights_kernel<false>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+  if (e != cudaSuccess) return e;
+  kernel<<<dim3(p.ntk, p.B * p.H), NT, SMEM_BYTES, st>>>(p);
   return cudaGetLastError();
 }
 

@@ -110,3 +110,15 @@ def test_cache_refusals():
     for kw, rc in ((dict(pos=None), V), (dict(pos=A + 4), AL), (dict(lse=None), V), (dict(w=None), V), (dict(first=200), V),
                    (dict(first=-1), V), (dict(dtype=_lib.F32), _lib.ERR_TYPE)):
         assert weights(**kw) == rc, kw
+
+
+def test_launches_report_a_refused_shared_memory_size():
+    """Every opt-in to more shared memory in the paged cache's sources hands its result on."""
+    import re
+
+    csrc = Path(__file__).resolve().parents[1] / "sisa_b200" / "csrc"
+    for name in ("paged_attn.cu", "paged_cache.cu", "key_weights.cu"):
+        text = (csrc / name).read_text()
+        calls = re.findall(r"^(.*)\bcudaFuncSetAttribute\(", text, flags=re.M)
+        assert calls and all(head.rstrip().endswith("=") for head in calls), name
+        assert len(re.findall(r"if \(e != cudaSuccess\) return e;", text)) >= len(calls), name
