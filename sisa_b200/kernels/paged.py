@@ -176,7 +176,7 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
     if fgate is not None and pages.f is None:
         raise ValueError("fgate is given but the pages hold no f plane")
     for name, t in (("g", g), ("fgate", fgate)):
-        if t is not None and (t.numel() != B * H or t.device != dev):
+        if t is not None and (t.numel() != B * H or t.shape[0] != B or t.device != dev):
             raise ValueError(f"{name} must be ({B}, {H}, 1) on {dev}, got {tuple(t.shape)} on {t.device}")
     if lam.shape != (H,) or lam.device != dev:
         raise ValueError(f"lam must have shape {(H,)} on {dev}, got {tuple(lam.shape)} on {lam.device}")
@@ -263,7 +263,7 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
     if z is not None:
         if pages.f is None:
             raise ValueError("z is given but the pages hold no f plane")
-        if z.numel() != B * H or z.device != dev:
+        if z.numel() != B * H or z.shape[0] != B or z.device != dev:
             raise ValueError(f"z must be ({B}, 1, {H}) on {dev}, got {tuple(z.shape)} on {z.device}")
         z2 = _f32(z)
         f = torch.empty_like(g)

@@ -139,3 +139,24 @@ def test_inputs_that_require_a_gradient_are_refused(cuda_dev):
                 fn(*a)
             with torch.no_grad():
                 fn(*a)
+
+
+def test_per_row_values_of_another_order_are_refused(cuda_dev):
+    """g, F and the forget logits as (H, B): as many values as are wanted, in the wrong order."""
+    from sisa_b200.kernels import paged as K
+
+    dev, B, H = cuda_dev, 3, 2
+    pages, table, rows, x = attn_case([40, 7, 12], H, 16, torch.bfloat16, dev, seed=1)
+    d = {n: t.to(dev) for n, t in x.items()}
+    ln = torch.tensor([40, 7, 12], dtype=torch.int32, device=dev)
+    proj, carry = torch.zeros(B, 1, 560, dtype=torch.bfloat16, device=dev), torch.zeros(B, H, 18, device=dev)
+    z, idle = torch.zeros(B, 1, H, device=dev), torch.full((B,), -1, dtype=torch.int32, device=dev)
+    args = (pages, table, ln, d["lam"])
+    want = K.paged_attention(d["q"], d["c"], d["gq"], d["fq"], *args)
+    assert torch.equal(want, K.paged_attention(d["q"], d["c"], d["gq"].view(B, H), d["fq"].view(B, 1, H), *args))
+    K.paged_append(proj, z.view(B, H), pages, table, idle, carry)
+    for g, f in ((d["gq"].transpose(0, 1), d["fq"]), (d["gq"], d["fq"].transpose(0, 1)), (d["gq"][:2], d["fq"])):
+        with pytest.raises(ValueError, match="must be"):
+            K.paged_attention(d["q"], d["c"], g, f, *args)
+    with pytest.raises(ValueError, match="must be"):
+        K.paged_append(proj, z.transpose(0, 2), pages, table, idle, carry)
