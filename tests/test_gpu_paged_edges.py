@@ -160,3 +160,98 @@ def test_per_row_values_of_another_order_are_refused(cuda_dev):
             K.paged_attention(d["q"], d["c"], g, f, *args)
     with pytest.raises(ValueError, match="must be"):
         K.paged_append(proj, z.transpose(0, 2), pages, table, idle, carry)
+
+
+# 13, 30 and 301 leave a ragged last group of four keys; the wide tables take the kernels that split the keys
+@pytest.mark.parametrize("S,wide", [(16, False), (16, True), (64, False), (64, True), (256, True)])
+def test_weights_are_written_in_used_slots_only(cuda_dev, S, wide):
+    """Unused slots hold a sentinel in both planes: in place and into a plane of its own, every used slot becomes
+    weight + share and no other value changes."""
+    from sisa_b200 import backends
+
+    lengths = [13, 0, 30, 301, 64, 1, 2 * S + 3]
+    pages, table, rows, x = attn_case(lengths, 3, S, torch.bfloat16, cuda_dev, seed=S)
+    t = widen(table) if wide else table
+    used = torch.zeros_like(pages.weight, dtype=torch.bool)
+    for i, n in enumerate(lengths):
+        if n:
+            put(used, table, i, torch.ones(pages.n_head, n, dtype=torch.bool))
+    pages.weight[~used] = 17.25
+    before = pages.weight.clone()
+    out = torch.full_like(before, -3.5)
+    y0, lse0 = call(pages, t, lengths, x, cuda_dev, accumulate=True, weight_out=out)
+    backends.check_status(cuda_dev)
+    assert torch.equal(pages.weight, before) and bool((out[~used] == -3.5).all())
+    y1, lse1 = call(pages, t, lengths, x, cuda_dev, accumulate=True)
+    backends.check_status(cuda_dev)
+    assert bool((pages.weight[~used] == 17.25).all()) and torch.equal(pages.weight[used], out[used])
+    assert torch.equal(y0, y1) and torch.equal(lse0, lse1)
+    for i, want in enumerate(attn_truth(rows, lengths, x)):
+        if want is not None:
+            check_row(y0[i, :, 0].cpu(), lse0[i].cpu(), get(out, table, i, lengths[i]), rows[i], want)
+
+
+@pytest.mark.parametrize("units,budget,S", [((1, 1), 4097, 16), ((2, 2), 8192, 64), ((1, 3), 5003, 128), ((3, 1), 40961, 256)])
+def test_evict_by_clusters_of_eight(cuda_dev, units, budget, S):
+    """Few units with a large budget: eight blocks share one, their minima meet in the first. The least weight lies in
+    each block's part once, and ties across blocks go to the lowest slot."""
+    from sisa_b200 import backends
+    from sisa_b200.kernels.paged import paged_evict
+    from tests.test_gpu_paged import make_pages, make_table
+
+    B, H = units
+    gen = torch.Generator().manual_seed(budget)
+    table, P = make_table([budget] * B, S, 3, cuda_dev)
+    pages = make_pages(P, H, S, torch.bfloat16, cuda_dev)
+    tok = torch.stack([torch.stack([torch.randperm(budget, generator=gen) for _ in range(H)]) for _ in range(B)])
+    w = torch.rand(B, H, budget, generator=gen) + 1.0
+    for b in range(B):
+        put(pages.token, table, b, tok[b].to(torch.int32))
+    recent = 50
+    pos = torch.full((B,), budget, dtype=torch.int32, device=cuda_dev)
+    old = tok < budget - recent
+    spots = [0, 3, 1023, 1024, 2047, 2048, 3500, 4095, budget - 1] + [k * 1024 + 5 for k in range(budget // 1024)]
+    for j in spots:
+        v = w.clone()
+        v[..., j] = 0.5
+        v[..., j + 700:j + 702] = 0.5                     # ties further on
+        for b in range(B):
+            put(pages.weight, table, b, v[b])
+        got = paged_evict(pages, table, pos, budget, recent).cpu().long()
+        backends.check_status(cuda_dev)
+        masked = v.masked_fill(~old, math.inf)
+        least = masked.min(-1, keepdim=True).values
+        first = (masked == least).to(torch.int8).argmax(-1)          # the lowest slot of the least weight
+        assert torch.equal(got, first), j
+
+
+@pytest.mark.parametrize("L,keep,recent,S", [(5, 3, 0, 16), (700, 100, 37, 64), (1500, 1499, 1, 32)])
+def test_fill_with_a_choice_in_fp16(cuda_dev, L, keep, recent, S):
+    from sisa_b200 import backends
+    from sisa_b200.kernels.paged import paged_fill
+    from tests.test_gpu_paged import fill_truth, make_pages, make_table, prompt
+
+    B, H = 2, 3
+    q, k, v, c, b, pos, lam, lse = prompt(B, H, L, torch.float16, cuda_dev, seed=L)
+    w = torch.rand(B, H, L, generator=torch.Generator().manual_seed(L))
+    w[1, 1] = (w[1, 1] * 4).round()
+    table, P = make_table([keep] * B, S, L, cuda_dev)
+    pages = make_pages(P, H, S, torch.float16, cuda_dev, fill=0.25)
+    pages.weight.fill_(7.5)
+    pages.token.fill_(-9)
+    g, f = pos[:, :, 0, :L], pos[:, :, 1, :L]
+    assert paged_fill(pages, table, k, v, b, g, f, weight=w.to(cuda_dev), keep=keep, recent=recent) == keep
+    backends.check_status(cuda_dev)
+    idx = fill_truth(w, keep, recent)
+    used = torch.zeros_like(pages.weight, dtype=torch.bool)
+    for i in range(B):
+        put(used, table, i, torch.ones(H, keep, dtype=torch.bool))
+        at = idx[i]
+        assert torch.equal(get(pages.token, table, i, keep).long(), at)
+        for plane, src in ((pages.k, k), (pages.v, v), (pages.b, b)):
+            assert torch.equal(get(plane, table, i, keep), src[i].cpu().gather(1, at.unsqueeze(-1).expand(-1, -1, src.shape[-1])))
+        for plane, src in ((pages.g, g), (pages.f, f), (pages.weight, w)):
+            assert torch.equal(get(plane, table, i, keep), src[i].cpu().gather(1, at))
+    for plane, value in ((pages.k, 0.25), (pages.v, 0.25), (pages.b, 0.25), (pages.g, 0.25), (pages.f, 0.25), (pages.weight, 7.5),
+                         (pages.token, -9)):
+        assert bool((plane[~used] == value).all())
