@@ -250,7 +250,7 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
             raise ValueError(f"carry must be a contiguous {(B, H, CARRY)} fp32 tensor on {dev}, got {tuple(t.shape)} "
                              f"{t.dtype} on {t.device}")
     sb, _, sl = proj.stride()
-    if sl != 1 or proj.data_ptr() % 16 or (sb % 8 and B > 1):
+    if sl != 1 or proj.data_ptr() % 16 or (B > 1 and (sb % 8 or sb < width)):    # (sb < width: rows shared or overlapping)
         proj = proj.contiguous()
         sb = width
         if B > 1 and sb % 8:                    # rows of odd width: q's rows are read in 16-byte units
@@ -305,7 +305,9 @@ def attention_key_weights(q: Tensor, k: Tensor, c: Tensor, b: Tensor, pos: Tenso
     dev = q.device
     if any(t.device != dev for t in (k, c, b, pos, lam, lse)) or not q.is_cuda:
         raise ValueError("attention_key_weights takes CUDA tensors on one device")
-    q, k, c, b, lse = _operand(q), _operand(k), _operand(c), _operand(b), lse.contiguous()
+    # (a tensor map has no stride of 0: operands shared by sequences or heads are copied)
+    q, k, c, b = (_operand(t if t.stride(0) and t.stride(1) else t.contiguous()) for t in (q, k, c, b))
+    lse = lse.contiguous()
     w = lse.new_empty((B, H, L))
     rc = lib.sisa_attn_key_weights(*map(_lib.view4_bytes, (q, k, c, b)), pos.data_ptr(), lam.data_ptr(), lse.data_ptr(), B,
                                    H, L, int(first_query), code, w.data_ptr(), backends.status_word(dev).data_ptr(),

@@ -255,3 +255,63 @@ def test_fill_with_a_choice_in_fp16(cuda_dev, L, keep, recent, S):
     for plane, value in ((pages.k, 0.25), (pages.v, 0.25), (pages.b, 0.25), (pages.g, 0.25), (pages.f, 0.25), (pages.weight, 7.5),
                          (pages.token, -9)):
         assert bool((plane[~used] == value).all())
+
+
+def test_queries_shared_by_broadcasting(cuda_dev):
+    """A query row that several sequences share through a stride of 0 gives what copies of it give."""
+    from sisa_b200.kernels import paged as K
+
+    dev, lengths = cuda_dev, [40, 300, 77]
+    pages, table, rows, x = attn_case(lengths, 2, 16, torch.bfloat16, dev, seed=5)
+    ln = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    q, c = x["q"][:1].to(dev).expand(3, 2, 1, 64), x["c"][:1, :1].to(dev).expand(3, 2, 1, 32)
+    g, f = x["gq"][:1].to(dev).expand(3, 2, 1), x["fq"][:1].to(dev).expand(3, 2, 1)
+    a = K.paged_attention(q, c, g, f, pages, table, ln, x["lam"].to(dev))
+    b = K.paged_attention(q.contiguous(), c.contiguous(), g.contiguous(), f.contiguous(), pages, table, ln, x["lam"].to(dev))
+    assert torch.equal(a, b)
+
+
+def test_a_prompt_shared_by_broadcasting(cuda_dev):
+    from sisa_b200 import backends
+    from sisa_b200.kernels import paged as K
+    from tests.test_gpu_paged import make_pages, make_table, prompt
+
+    L = 130
+    q, k, v, c, b, pl, lam, lse = prompt(1, 2, L, torch.bfloat16, cuda_dev, seed=2)
+    w = K.attention_key_weights(q, k, c, b, pl, lam, lse)
+    q3, k3, c3, b3, l3 = (t.expand(3, *t.shape[1:]) for t in (q, k, c, b, lse))
+    assert torch.equal(K.attention_key_weights(q3, k3, c3, b3, pl.repeat(3, 1, 1, 1), lam, l3), w.expand(3, 2, L))
+    heads = K.attention_key_weights(q, k[:, :1].expand(1, 2, L, 64), c, b, pl, lam, lse)       # keys shared by the heads
+    assert torch.equal(heads, K.attention_key_weights(q, k[:, :1].repeat(1, 2, 1, 1), c, b, pl, lam, lse))
+    table, P = make_table([50] * 3, 32, 4, cuda_dev)
+    src = [t.expand(3, *t.shape[1:]) for t in (k, v, b, pl[:, :, 0, :L], pl[:, :, 1, :L], w)]
+    filled = [make_pages(P, 2, 32, torch.bfloat16, cuda_dev, fill=0.5) for _ in range(2)]
+    K.paged_fill(filled[0], table, *src[:5], weight=src[5], keep=50, recent=9)
+    src = [t.contiguous() for t in src]
+    K.paged_fill(filled[1], table, *src[:5], weight=src[5], keep=50, recent=9)
+    backends.check_status(cuda_dev)
+    for name in ("k", "v", "b", "g", "f", "weight", "token"):
+        assert torch.equal(getattr(filled[0], name), getattr(filled[1], name)), name
+
+
+@pytest.mark.parametrize("H", [2, 3])
+def test_a_projection_row_shared_by_broadcasting(cuda_dev, H):
+    """The same new token for three sequences, and rows that overlap."""
+    from sisa_b200 import backends
+    from sisa_b200.kernels import paged as K
+    from tests.test_gpu_paged import make_pages, make_table
+
+    dev, bf, n = cuda_dev, torch.bfloat16, 273 * H + 8
+    gen = torch.Generator().manual_seed(H)
+    flat = torch.randn(n + 32, generator=gen).to(bf).to(dev)
+    z, carry = torch.randn(1, 1, H, generator=gen).to(dev), torch.zeros(3, H, 18, device=dev)
+    pos = torch.tensor([5, 0, 49], dtype=torch.int32, device=dev)
+    table, P = make_table([50] * 3, 32, 4, dev)
+    for proj in (flat[:n].view(1, 1, n).expand(3, 1, n), flat.as_strided((3, 1, n), (16, n, 1))):
+        got = []
+        for p, zz in ((proj, z.expand(3, 1, H)), (proj.contiguous(), z.repeat(3, 1, 1))):
+            pages, co = make_pages(P, H, 32, bf, dev, fill=0.5), carry.clone()
+            out = K.paged_append(p, zz, pages, table, pos, co)
+            got.append([*out, co, pages.k, pages.v, pages.b, pages.g, pages.f, pages.weight, pages.token])
+        backends.check_status(dev)
+        assert all(torch.equal(s, t) for s, t in zip(*got))
