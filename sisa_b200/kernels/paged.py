@@ -123,7 +123,7 @@ def _operand(t: Tensor) -> Tensor:
     a, b, c, d = t.stride()
     if d == 1 and (a | b | c) % 8 == 0 and c > 0 and a >= 0 and b >= 0 and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)      # (contiguous() keeps a dense tensor where it is, aligned or not)
 
 
 def _f32(t: Tensor) -> Tensor:
@@ -251,7 +251,7 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
                              f"{t.dtype} on {t.device}")
     sb, _, sl = proj.stride()
     if sl != 1 or proj.data_ptr() % 16 or (B > 1 and (sb % 8 or sb < width)):    # (sb < width: rows shared or overlapping)
-        proj = proj.contiguous()
+        proj = proj.clone(memory_format=torch.contiguous_format)
         sb = width
         if B > 1 and sb % 8:                    # rows of odd width: q's rows are read in 16-byte units
             wide = proj.new_empty((B, 1, -(-width // 8) * 8))

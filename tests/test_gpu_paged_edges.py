@@ -315,3 +315,46 @@ def test_a_projection_row_shared_by_broadcasting(cuda_dev, H):
             got.append([*out, co, pages.k, pages.v, pages.b, pages.g, pages.f, pages.weight, pages.token])
         backends.check_status(dev)
         assert all(torch.equal(s, t) for s, t in zip(*got))
+
+
+def shifted(t, elements=4):
+    """A dense copy of t that starts off a 16-byte boundary."""
+    flat = torch.empty(t.numel() + 16, dtype=t.dtype, device=t.device)
+    out = flat[elements:elements + t.numel()].view(t.shape)
+    assert out.data_ptr() % 16
+    return out.copy_(t)
+
+
+def test_dense_operands_off_a_16_byte_boundary(cuda_dev):
+    from sisa_b200 import backends
+    from sisa_b200.kernels import paged as K
+    from tests.test_gpu_paged import make_pages, make_table, prompt
+
+    dev, bf, L = cuda_dev, torch.bfloat16, 70
+    pages, table, rows, x = attn_case([40], 2, 16, bf, dev, seed=5)
+    ln, d = torch.tensor([40], dtype=torch.int32, device=dev), {n: t.to(dev) for n, t in x.items()}
+    want = K.paged_attention(d["q"], d["c"], d["gq"], d["fq"], pages, table, ln, d["lam"])
+    got = K.paged_attention(shifted(d["q"]), shifted(d["c"]), shifted(d["gq"], 1), shifted(d["fq"], 1), pages, table, ln,
+                            shifted(d["lam"], 1))
+    assert torch.equal(got, want)
+    q, k, v, c, b, pl, lam, lse = prompt(2, 2, L, bf, dev, seed=2)
+    w = K.attention_key_weights(q, k, c, b, pl, lam, lse)
+    moved = [shifted(t) for t in (q, k, c, b)]
+    assert torch.equal(K.attention_key_weights(*moved, pl, shifted(lam, 1), shifted(lse, 1)), w)
+    table, P = make_table([50, 50], 32, 4, dev)
+    src, filled = [k, v, b, pl[:, :, 0, :L].contiguous(), pl[:, :, 1, :L].contiguous(), w], []
+    for move in (False, True):
+        pages = make_pages(P, 2, 32, bf, dev, fill=0.5)
+        s = [shifted(t, 1 if t.dtype == torch.float32 else 4) for t in src] if move else src
+        K.paged_fill(pages, table, *s[:5], weight=s[5], keep=50, recent=9)
+        filled.append(pages)
+    gen = torch.Generator().manual_seed(1)
+    proj, z = torch.randn(2, 1, 560, generator=gen).to(bf).to(dev), torch.randn(2, 1, 2, generator=gen).to(dev)
+    carry, pos = torch.zeros(2, 2, 18, device=dev), torch.tensor([7, 49], dtype=torch.int32, device=dev)
+    one = K.paged_append(proj, z, filled[0], table, pos, carry.clone())
+    for n in (1, 2):                                       # one row by itself too
+        two = K.paged_append(shifted(proj)[:n], shifted(z, 1)[:n], filled[1], table[:n], pos[:n], carry[:n].clone())
+        assert all(torch.equal(s[:n], t) for s, t in zip(one, two)) and two[0].data_ptr() % 16 == 0
+    backends.check_status(dev)
+    for name in ("k", "v", "b", "g", "f", "weight", "token"):
+        assert torch.equal(getattr(filled[0], name), getattr(filled[1], name)), name
