@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -114,12 +115,14 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 using CtxGetFn = CUresult (*)(CUcontext*);
 using CtxSetFn = CUresult (*)(CUcontext);
+using PtrAttrsFn = CUresult (*)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
 
-// cuCtxGetCurrent / cuCtxSetCurrent through the runtime's driver entry-point query (no link against
-// libcuda), resolved once; null if the driver does not offer them.
+// cuCtxGetCurrent / cuCtxSetCurrent / cuPointerGetAttributes through the runtime's driver entry-point query (no
+// link against libcuda), resolved once; null if the driver does not offer them.
 struct CtxFns {
   CtxGetFn get = nullptr;
   CtxSetFn set = nullptr;
+  PtrAttrsFn attrs = nullptr;
 };
 const CtxFns& ctx_fns() {
   static CtxFns f;
@@ -133,9 +136,16 @@ const CtxFns& ctx_fns() {
     if (cudaGetDriverEntryPoint("cuCtxSetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
         q == cudaDriverEntryPointSuccess)
       f.set = reinterpret_cast<CtxSetFn>(p);
+    if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      f.attrs = reinterpret_cast<PtrAttrsFn>(p);
   });
   return f;
 }
+
+// The primary context of each device that a bind() has made current.
+constexpr int kDevices = 64;
+std::atomic<CUcontext> g_primary[kDevices];
 
 int check_view(const sisa_view4* v, int elem_bytes, const char* name) {
   if (!v || !v->data) return fail(SISA_ERR_VALUE, "%s: null view", name);
@@ -188,13 +198,26 @@ int capi_check_view(const sisa_view4* v, int elem_bytes, const char* name) { ret
 int capi_check_dtype(int dtype) { return check_dtype(dtype); }
 
 int DeviceScope::bind(const void* ptr) {
+  const CtxFns& f = ctx_fns();
+  CUcontext cur = nullptr;
+  // The usual case costs two driver calls: the owner's primary context is current already.
+  if (f.get && f.attrs && f.get(&cur) == CUDA_SUCCESS && cur) {
+    unsigned type = 0;
+    int owner = -1;
+    CUpointer_attribute what[2] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+    void* out[2] = {&type, &owner};
+    if (f.attrs(2, what, out, reinterpret_cast<CUdeviceptr>(ptr)) == CUDA_SUCCESS && type == CU_MEMORYTYPE_DEVICE &&
+        owner >= 0 && owner < kDevices && g_primary[owner].load(std::memory_order_relaxed) == cur) {
+      device_ = owner;
+      return SISA_OK;
+    }
+  }
   cudaPointerAttributes a;
   cudaError_t e = cudaPointerGetAttributes(&a, ptr);
   if (e != cudaSuccess) return cuda_fail(e, "cudaPointerGetAttributes");
   if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
     return fail(SISA_ERR_VALUE, "tensor data is not device memory");
-  const CtxFns& f = ctx_fns();
-  CUcontext cur = nullptr;
+  cur = nullptr;
   if (f.get && f.set && f.get(&cur) == CUDA_SUCCESS) {
     prev_ = cur;
     bound_ = true;
@@ -202,6 +225,9 @@ int DeviceScope::bind(const void* ptr) {
   e = cudaSetDevice(a.device);   // makes the device's primary context current on this thread
   if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
   device_ = a.device;
+  CUcontext now = nullptr;
+  if (a.device < kDevices && f.get && f.get(&now) == CUDA_SUCCESS)
+    g_primary[a.device].store(now, std::memory_order_relaxed);
   return SISA_OK;
 }
 

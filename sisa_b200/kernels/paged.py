@@ -64,14 +64,16 @@ class KeyPages:
                 raise TypeError(f"plane {name} must be {dt}, got {t.dtype}")
         if any(t is not None and t.device != k.device for t in (v, b, g, f, weight, token)):
             raise ValueError("all pages must lie on one device")
-        _refuse_grad("KeyPages", k, v, b, g, f, weight)
+        if torch.is_grad_enabled():
+            _refuse_grad("KeyPages", k, v, b, g, f, weight)
         self.k, self.v, self.b, self.g, self.f, self.weight, self.token = k, v, b, g, f, weight, token
         self.n_pages, self.n_head, self.page_size = P, H, S
         self.dtype, self.device = k.dtype, k.device
         c = _lib.Pages(k.data_ptr(), v.data_ptr(), b.data_ptr(), g.data_ptr(), _lib.ptr(f), _lib.ptr(weight),
                              _lib.ptr(token), k.stride(0), k.stride(1), v.stride(0), v.stride(1), b.stride(0), b.stride(1),
                              g.stride(0), g.stride(1), P, S)
-        self.cbytes = bytes(c)                  # the struct every call passes
+        self.cbytes = bytes(c)                  # the struct every call passes, and its device's status word
+        self.status = backends.status_word(self.device).data_ptr() if k.is_cuda else None
         self.ws_bytes: dict[tuple, int] = {}    # workspace sizes of the tables seen
 
     @classmethod
@@ -89,12 +91,11 @@ class KeyPages:
 
 
 def _refuse_grad(what: str, *tensors: Tensor | None) -> None:
-    """These operators serve; none has a backward. Where a gradient would be recorded for an input, raise rather than
-    return a result that has lost it."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{what} has no backward: call it under torch.no_grad() or with detached inputs")
+    """These operators serve; none has a backward. In grad mode (the caller looks) an input that requires a gradient
+    raises, rather than a result that has lost it being returned."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{what} has no backward: call it under torch.no_grad() or with detached inputs")
 
 
 def _table(pages: KeyPages, table: Tensor, B: int) -> tuple[int, int, int]:
@@ -157,7 +158,8 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
     ``weight_out`` = ``pages.weight`` + share where that plane is given (used slots only). No two rows may then
     share a page: both would add to the same weights, and one of the shares could be lost."""
     B, H = _check_query(q, c, pages)
-    _refuse_grad("paged_attention", q, c, g, fgate, lam, weight_out)
+    if torch.is_grad_enabled():
+        _refuse_grad("paged_attention", q, c, g, fgate, lam, weight_out)
     lib = _lib.load()
     dev = pages.device
     tp, tsb, mp = _table(pages, block_table, B)
@@ -197,7 +199,7 @@ def paged_attention(q: Tensor, c: Tensor, g: Tensor, fgate: Tensor | None, pages
                              pages.cbytes, tp, tsb, mp, lp, lam.data_ptr(), B, H, pages.dtype_code, _lib.view4_bytes(y),
                              None if lse is None else lse.data_ptr(), None if wo is None else wo.data_ptr(),
                              None if ws is None else ws.data_ptr(),
-                             backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+                             pages.status, _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_attn")
     backends.after_call(dev)
     return (y, lse) if return_lse else y
@@ -213,7 +215,7 @@ def paged_evict(pages: KeyPages, block_table: Tensor, position: Tensor, budget: 
     dev = pages.device
     slots = position.new_empty((B, H))
     rc = _lib.load().sisa_paged_evict(pages.cbytes, tp, tsb, mp, pp, B, H, int(budget), int(recent), slots.data_ptr(),
-                                      backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+                                      pages.status, _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_evict")
     backends.after_call(dev)
     return slots
@@ -239,7 +241,8 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
         raise TypeError(f"projection dtype {proj.dtype} differs from the pages' {pages.dtype}")
     if proj.device != dev:
         raise ValueError(f"proj is on {proj.device}, the pages on {dev}")
-    _refuse_grad("paged_append", proj, z, carry, carry_out)
+    if torch.is_grad_enabled():
+        _refuse_grad("paged_append", proj, z, carry, carry_out)
     tp, tsb, mp = _table(pages, block_table, B)
     pp = _rows(position, (B,), "position", pages)
     sp = None if slots is None else _rows(slots, (B, H), "slots", pages)
@@ -270,7 +273,7 @@ def paged_append(proj: Tensor, z: Tensor | None, pages: KeyPages, block_table: T
         zp, fp = z2.data_ptr(), f.data_ptr()
     rc = _lib.load().sisa_paged_append(proj.data_ptr(), sb if B > 1 else width, zp, H, pages.cbytes, tp, tsb, mp, pp, sp,
                                        int(budget or 0), B, H, pages.dtype_code, carry.data_ptr(), co.data_ptr(),
-                                       c.data_ptr(), g.data_ptr(), fp, lp, backends.status_word(dev).data_ptr(),
+                                       c.data_ptr(), g.data_ptr(), fp, lp, pages.status,
                                        _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_append")
     backends.after_call(dev)
@@ -291,7 +294,8 @@ def attention_key_weights(q: Tensor, k: Tensor, c: Tensor, b: Tensor, pos: Tenso
                          f"{tuple(k.shape)}, {tuple(c.shape)} and {tuple(b.shape)}")
     if any(t.dtype != q.dtype for t in (k, c, b)):
         raise TypeError(f"q, k, c and b differ in dtype: {q.dtype}, {k.dtype}, {c.dtype}, {b.dtype}")
-    _refuse_grad("attention_key_weights", q, k, c, b, pos, lam, lse)
+    if torch.is_grad_enabled():
+        _refuse_grad("attention_key_weights", q, k, c, b, pos, lam, lse)
     lib = _lib.load()
     code = _lib.dtype_code(q.dtype)
     if pos.shape != (B, H, 4, lib.sisa_pos_len(L)) or not pos.is_contiguous() or pos.dtype != torch.float32:
@@ -331,7 +335,8 @@ def paged_fill(pages: KeyPages, block_table: Tensor, k: Tensor, v: Tensor, b: Te
                          f"{tuple(v.shape)} and {tuple(b.shape)}")
     if k.dtype != pages.dtype or v.dtype != pages.dtype or b.dtype != pages.dtype:
         raise TypeError(f"k, v and b must be {pages.dtype} like the pages, got {k.dtype}, {v.dtype}, {b.dtype}")
-    _refuse_grad("paged_fill", k, v, b, g, fgate, weight)
+    if torch.is_grad_enabled():
+        _refuse_grad("paged_fill", k, v, b, g, fgate, weight)
     dev = pages.device
     for t in (k, v, b, g, fgate, weight):
         if t is not None and t.device != dev:
@@ -354,7 +359,7 @@ def paged_fill(pages: KeyPages, block_table: Tensor, k: Tensor, v: Tensor, b: Te
     fs = (0, 0) if fgate is None else fgate.stride()[:2]
     rc = lib.sisa_paged_fill(pages.cbytes, tp, tsb, mp, *map(_lib.view4_bytes, (k, v, b)), g.data_ptr(), g.stride(0),
                              g.stride(1), _lib.ptr(fgate), *fs, _lib.ptr(weight), B, H, L, keep, int(recent), ws.data_ptr(),
-                             backends.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+                             pages.status, _lib.stream_ptr(dev))
     _lib.check(rc, "sisa_paged_fill")
     backends.after_call(dev)
     return keep
