@@ -358,3 +358,39 @@ def test_dense_operands_off_a_16_byte_boundary(cuda_dev):
     backends.check_status(dev)
     for name in ("k", "v", "b", "g", "f", "weight", "token"):
         assert torch.equal(getattr(filled[0], name), getattr(filled[1], name)), name
+
+
+def test_calls_from_a_thread_without_a_context(cuda_dev):
+    """A host thread that has not touched CUDA: the call makes the owner's context current for itself and leaves the
+    thread as it was; the thread that has it current keeps it."""
+    import ctypes
+    import threading
+
+    from sisa_b200 import _lib, backends
+    from sisa_b200.kernels import paged as K
+
+    pages, table, rows, x = attn_case([128], 2, 16, torch.bfloat16, cuda_dev, seed=3)
+    put(pages.token, table, 0, torch.arange(128).expand(2, 128).to(torch.int32).contiguous())
+    pos = torch.tensor([128], dtype=torch.int32, device=cuda_dev)
+    want = K.paged_evict(pages, table, pos, 128, 16)
+    slots, lib, driver = torch.zeros_like(want), _lib.load(), ctypes.CDLL("libcuda.so.1")
+    args = (pages.cbytes, table.data_ptr(), table.shape[1], table.shape[1], pos.data_ptr(), 1, 2, 128, 16, slots.data_ptr(),
+            pages.status, None)
+    torch.cuda.synchronize(cuda_dev)
+
+    def current():
+        ctx = ctypes.c_void_p()
+        assert driver.cuCtxGetCurrent(ctypes.byref(ctx)) == 0
+        return ctx.value
+
+    seen = []
+    thread = threading.Thread(target=lambda: seen.extend([current(), lib.sisa_paged_evict(*args), current(),
+                                                          lib.sisa_paged_evict(*args), current()]))
+    thread.start()
+    thread.join()
+    assert seen == [None, 0, None, 0, None]
+    torch.cuda.synchronize(cuda_dev)
+    assert torch.equal(slots, want)
+    here = current()
+    assert here is not None and lib.sisa_paged_evict(*args) == 0 and current() == here
+    backends.check_status(cuda_dev)
