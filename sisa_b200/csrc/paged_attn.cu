@@ -20,8 +20,9 @@
 // CTA, that paged_join_kernel merges in order (deterministic, no atomics). With weights, the scores are kept
 // in the workspace (4 bytes per key) and paged_weights_kernel adds the shares once lse is known.
 //
-// Measured (B200, a copy moves 6.55 TB/s): 64 sequences of 8192 keys x 16 heads 403 us = 6.84 TB/s, with weights
-// 461 us = 6.11 TB/s; one of 131,071 keys x 16 heads 120 us = 5.75 TB/s, of which about 10 us are start-up and join.
+// Measured (B200, a copy moves 6.55 TB/s): 64 sequences of 8192 keys x 16 heads 404 us = 6.81 TB/s, with weights
+// 455-468 us = 6.1 TB/s; one of 131,071 keys x 16 heads 118-121 us = 5.7 TB/s, of which about 10 us are start-up and
+// join.
 // Ten warps per SM with two stages each: four warps with five stages (one CTA per SM) took 504 us on the first
 // case before the waves, since a lone warp per scheduler hides none of its own latency.
 #include <cuda_runtime.h>
@@ -651,10 +652,12 @@ cudaError_t launch_after(K kernel, dim3 grid, int threads, cudaStream_t st, cons
 
 template <bool kHalf>
 cudaError_t launch(const PagedAttnParams& p, cudaStream_t st) {
-  // Short tables: one launch and no join. 16 heads, one CTA per unit against the split (us, without / with
-  // weights): 1 x 256 keys 10.3 / 12.3 against 15.4 / 15.4, 8 x 256 12.3 / 14.2 against 18.5 / 19.5, 64 x 256
-  // 32.8 / 36.9 against 33.9 / 35.9; at 1024 keys 1 x 18.4 / 21.3 against 15.4 / 17.5, 64 x 69.6 / 84.0 against
-  // 72.7 / 74.9.
+  // Short tables: one launch and no join. 16 heads, one CTA per unit against the split (us in a captured graph, L2
+  // flushed before each, without / with weights): 256 keys, 1 x 12.2 / 12.3 against 14.4 / 15.3, 16 x 14.4 / 16.4
+  // against 18.5 / 20.5, 64 x 32.8 / 37.0 against 30.6 / 33.8; 512 keys, 1 x 14.3 / 16.4 against 14.3 / 14.4, 16 x
+  // 18.4 / 20.5 against 22.6 / 22.6, 32 x 28.7 / 32.8 against 28.7 / 30.7, 64 x 47.1 / 55.3 against 43.0 / 47.1; 1024
+  // keys, 1 x 18.4 / 21.3 against 15.4 / 17.5. So it pays up to about 256 units and costs up to 8 us at 1024 units.
+  // The rule sees the table, not the lengths: 77 keys x 8 heads take 10.2 under a table of 512 and 14.4 under one of 4096.
   const bool unit = p.max_keys <= UNIT_KEYS;
   auto* main = p.weight_out ? (unit ? paged_attn_kernel<kHalf, true, true> : paged_attn_kernel<kHalf, true, false>)
                             : (unit ? paged_attn_kernel<kHalf, false, true> : paged_attn_kernel<kHalf, false, false>);

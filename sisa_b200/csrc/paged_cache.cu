@@ -34,11 +34,12 @@ __device__ __forceinline__ unsigned long long cluster_load(const unsigned long l
 // newest (token < position - recent), the lowest slot where several weigh the same; -1 while the sequence
 // holds fewer than budget keys. (weight, slot) is one 64-bit number, so the minimum does not depend on the
 // order in which it is taken.
-// HBM-bound: 8 bytes per key. A thread takes four slots at a time (16-byte loads of both planes), two such
+// Bound by memory: 8 bytes per key. A thread takes four slots at a time (16-byte loads of both planes), two such
 // steps in flight; a cluster of blocks shares a unit when there are few units, and its first block takes
-// the minimum over the others' through distributed shared memory. 64 x 16 units of 8192 slots (67 MB): 13.5 us;
-// one step in flight 14.5 us; with 64-bit comparisons per slot 16.6 us (four steps: 20.6 us); the first version,
-// one slot per thread and step, 38 us.
+// the minimum over the others' through distributed shared memory. 64 x 16 units of 8192 slots (67 MB): 13.4 us where
+// the planes are still in L2, 18.1 us = 3.7 TB/s where five other layers' planes have passed in between. In L2, one
+// step in flight 14.5 us; with 64-bit comparisons per slot 16.6 us (four steps: 20.6 us); the first version, one
+// slot per thread and step, 38 us.
 constexpr int EVICT_CLUSTER = 8;                 // portable cluster size
 __global__ void __launch_bounds__(NT) paged_evict_kernel(PagedEvictParams p) {
   const int cs = cluster_blocks(), rank = blockIdx.x % cs;
@@ -109,8 +110,8 @@ __global__ void __launch_bounds__(NT) paged_evict_kernel(PagedEvictParams p) {
 // One warp per (batch, head): the new token's recurrences g' = g - softplus(alpha), F' = F + logsigmoid(z),
 // Phi' = Phi + theta, the rotation of c and b by Phi' (fp32, torch's separate products, one rounding), and
 // the write of its key into one slot of the sequence's pages. An idle row (position < 0) keeps its state,
-// writes no key and leaves zeros on the query side. Bound by latency: about 1 KB per (sequence, head), 5.5 us
-// for one sequence and 6.2 us for 64 x 16 heads, most of it the chain position -> page -> slot.
+// writes no key and leaves zeros on the query side. Bound by latency: about 1 KB per (sequence, head), 5.5-7 us
+// for one sequence and for 64 x 16 heads, most of it the chain position -> page -> slot.
 template <bool kHalf>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) {
   const int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
