@@ -7,7 +7,8 @@
  * stream that is passed in. Kernels never trap; run-time conditions are OR-ed into *status
  * (SISA_ST_* bits) and left for the caller to read. Every entry point that launches makes the device
  * that owns its data current for the length of the call and gives the calling thread back its previous
- * context before it returns (data in host memory is refused); the stream must belong to that device.
+ * context before it returns (a thread without one may keep its current device's); data in host memory is
+ * refused, and the stream must belong to the data's device.
  *
  * Reference interfaces (tlstngud/sisa, paths inside that project) that each entry point
  * replaces are cited beside it.

@@ -217,8 +217,12 @@ int DeviceScope::bind(const void* ptr) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaPointerGetAttributes");
   if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
     return fail(SISA_ERR_VALUE, "tensor data is not device memory");
+  // A thread without a context whose current device owns the data is left with that device's context, as after any
+  // call of the runtime: libraries that it calls next look for one.
   cur = nullptr;
-  if (f.get && f.set && f.get(&cur) == CUDA_SUCCESS) {
+  int device = -1;
+  if (f.get && f.set && f.get(&cur) == CUDA_SUCCESS &&
+      (cur || cudaGetDevice(&device) != cudaSuccess || device != a.device)) {
     prev_ = cur;
     bound_ = true;
   }

@@ -15,8 +15,8 @@ int capi_check_view(const sisa_view4* v, int elem_bytes, const char* name);
 int capi_check_dtype(int dtype);
 
 // Makes the device that owns an entry point's data current on the calling thread for the length of
-// the call. The destructor gives the thread back the context it had before bind() (or none), so an
-// entry point never changes its caller's current device. Tensor-map encoding needs a current context,
+// the call. The destructor gives the thread back the context it had before bind() (or none, where its
+// current device is another one), so an entry point never changes its caller's current device. Tensor-map encoding needs a current context,
 // which a thread that has not touched CUDA yet (an autograd worker, a foreign host thread) lacks.
 class DeviceScope {
  public:

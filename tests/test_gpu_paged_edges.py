@@ -361,8 +361,8 @@ def test_dense_operands_off_a_16_byte_boundary(cuda_dev):
 
 
 def test_calls_from_a_thread_without_a_context(cuda_dev):
-    """A host thread that has not touched CUDA: the call makes the owner's context current for itself and leaves the
-    thread as it was; the thread that has it current keeps it."""
+    """A host thread that has not touched CUDA gets the context of its current device, here the owner's, as from any
+    runtime call; a thread that has it current keeps it."""
     import ctypes
     import threading
 
@@ -388,9 +388,9 @@ def test_calls_from_a_thread_without_a_context(cuda_dev):
                                                           lib.sisa_paged_evict(*args), current()]))
     thread.start()
     thread.join()
-    assert seen == [None, 0, None, 0, None]
+    here = current()
+    assert here is not None and seen == [None, 0, here, 0, here]
     torch.cuda.synchronize(cuda_dev)
     assert torch.equal(slots, want)
-    here = current()
-    assert here is not None and lib.sisa_paged_evict(*args) == 0 and current() == here
+    assert lib.sisa_paged_evict(*args) == 0 and current() == here
     backends.check_status(cuda_dev)
