@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(NT, 3) key_weights_kernel(const __grid_constan
     auto lse_at = [&](int i) { return i < L ? __ldg(lse + i) : 0.f; };
     float f0 = f_at(i_begin + lane), f1 = f_at(i_begin + lane + 32);
     float n0 = lse_at(i_begin + lane), n1 = lse_at(i_begin + lane + 32);
-    for (int n = 0; n < ntiles; ++n) {
+    int n = 0;
+    for (; n < ntiles; ++n) {
       const int s = n % NSTAGE, i0 = i_begin + n * BQ;
       if (n >= NSTAGE && !warp_wait<true>(BAR(B_QE + s), ((n / NSTAGE) - 1) & 1, p.status)) break;
       const uint32_t st = stage_addr(s);
@@ -118,12 +119,17 @@ __global__ void __launch_bounds__(NT, 3) key_weights_kernel(const __grid_constan
       n0 = lse_at(i0 + BQ + lane);                 // the next tile's, in flight while this warp waits
       n1 = lse_at(i0 + BQ + lane + 32);
     }
+    if (n < ntiles) {                              // a wait ran out: let the copies in flight land before leaving
+      warp_wait<true>(BAR(B_K), 0, p.status);
+      for (int m = n - NSTAGE; m < n; ++m) warp_wait<true>(BAR(B_QF + m % NSTAGE), (m / NSTAGE) & 1, p.status);
+    }
   } else if (warp == NCW + 1) {
     // ------------------------------------------------------------------ UMMA issuer
     if (lane == 0) {
       constexpr uint32_t idesc = make_idesc(128, 64, kHalf ? 0 : 1, 0, 0);
-      bool ok = mbar_wait<true>(BAR(B_K), 0, p.status);
-      for (int n = 0; ok && n < ntiles; ++n) {
+      const bool ok = mbar_wait<true>(BAR(B_K), 0, p.status);
+      int n = 0;
+      for (; ok && n < ntiles; ++n) {
         const int s = n % NSTAGE;
         if (!mbar_wait<true>(BAR(B_QF + s), (n / NSTAGE) & 1, p.status)) break;
         if (n >= 1 && !mbar_wait<true>(BAR(B_SE), (n - 1) & 1, p.status)) break;
@@ -137,6 +143,8 @@ __global__ void __launch_bounds__(NT, 3) key_weights_kernel(const __grid_constan
         umma_commit(BAR(B_SF));
         umma_commit(BAR(B_QE + s));
       }
+      // (the same for the UMMAs, whose tensor memory is freed below)
+      if (n < ntiles && n > 0) mbar_wait<true>(BAR(B_SF), (n - 1) & 1, p.status);
     }
   } else {
     // ------------------------------------------------------------------ compute
